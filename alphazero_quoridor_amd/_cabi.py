@@ -19,7 +19,7 @@ LIB_PATH = os.path.join(_HERE, "libqzero_hip.so")
 CSRC = os.path.join(_HERE, "csrc")
 HEADER = os.path.join(os.path.dirname(_HERE), "include", "qz_abi.h")
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 N_ACTIONS = 140
 PLANES = 26 * 81
 MASK_WORDS = 5
@@ -142,9 +142,30 @@ class qz_nn_weights(C.Structure):
     ]
 
 
+class qz_policy_rows(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("n", C.c_int64), ("n_actions", C.c_int32), ("dtype", C.c_int32),
+                ("actions", C.c_void_p), ("legal", C.c_void_p), ("legal_ld", C.c_int64), ("legal_kind", C.c_int32)]
+
+
+class qz_policy_terms(C.Structure):
+    _fields_ = [("advantages", C.c_void_p), ("old_logp", C.c_void_p), ("ref_logp", C.c_void_p), ("weights", C.c_void_p),
+                ("ref_logits", C.c_void_p), ("ref_ld", C.c_int64), ("clip_low", C.c_float), ("clip_high", C.c_float),
+                ("kl_coef", C.c_float), ("entropy_coef", C.c_float)]
+
+
+class qz_matrix(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("update", C.c_void_p), ("ld", C.c_int64), ("out", C.c_void_p),
+                ("out_ld", C.c_int64), ("momentum", C.c_void_p), ("param", C.c_void_p), ("scale", C.c_float)]
+
+
+class qz_muon_opts(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("nesterov", C.c_int32), ("lr_dev", C.c_void_p)]
+
+
 def build(force: bool = False) -> str:
     """Compile libqzero_hip.so for gfx950 with hipcc (cross-compiles without a GPU)."""
-    srcs = [os.path.join(CSRC, f) for f in ("qz_kernels.hip", "qz_abi.hip", "qz_nn.hip", "qz_conv.hip", "qz_rules.h", "qz_movegen_pool.h", "qz_path_rows.h", "qz_device.h")] + [HEADER]
+    srcs = [os.path.join(CSRC, f) for f in ("qz_kernels.hip", "qz_abi.hip", "qz_nn.hip", "qz_conv.hip", "qz_policy.hip", "qz_ortho.hip", "qz_rules.h", "qz_movegen_pool.h",
+                                           "qz_path_rows.h", "qz_rows.h", "qz_device.h", "qz_policy.h", "qz_ortho.h")] + [HEADER]
     stale = force or not os.path.exists(LIB_PATH) or any(os.path.getmtime(s) > os.path.getmtime(LIB_PATH) for s in srcs)
     if stale:
         subprocess.check_call(["make", "-C", CSRC, "-s"])
@@ -205,6 +226,14 @@ _SIGNATURES = {
     "qz_selfplay_misses": (C.c_int, [_P, C.POINTER(qz_boards), C.POINTER(_P), C.POINTER(_P), C.POINTER(_P), C.POINTER(_P)]),
     "qz_memo_flush": (C.c_int, [_P, _P]),
     "qz_nn_head": (C.c_int, [_P, C.c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_float, _P]),
+    "qz_policy_workspace": (C.c_int64, [C.c_int64, C.c_int]),
+    "qz_action_logp": (C.c_int, [C.POINTER(qz_policy_rows), _P, _P, _P, _P, C.c_int64, _P]),
+    "qz_action_logp_backward": (C.c_int, [C.POINTER(qz_policy_rows), _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "qz_policy_loss": (C.c_int, [C.POINTER(qz_policy_rows), C.POINTER(qz_policy_terms), _P, _P, _P, _P, _P, C.c_int64, _P, C.c_int64, _P]),
+    "qz_policy_loss_backward": (C.c_int, [C.POINTER(qz_policy_rows), C.POINTER(qz_policy_terms), _P, C.c_int, _P, C.c_int64, _P, C.c_int64, _P]),
+    "qz_orthogonalize_workspace": (C.c_int64, [C.POINTER(qz_matrix), C.c_int]),
+    "qz_orthogonalize": (C.c_int, [C.POINTER(qz_matrix), C.c_int, C.c_int, C.c_int, _P, C.c_int64, _P]),
+    "qz_muon_step": (C.c_int, [C.POINTER(qz_matrix), C.c_int, C.c_int, C.c_int, C.POINTER(qz_muon_opts), _P, C.c_int64, _P]),
     "qz_selftest_sqrt": (C.c_int, [_P, C.c_int, _P]),
 }
 

@@ -13,6 +13,8 @@
 
 #include "../../include/qz_abi.h"
 #include "qz_device.h"
+#include "qz_ortho.h"
+#include "qz_policy.h"
 
 namespace qzl {
 hipError_t movegen_encode(const uint64_t*, const uint64_t*, const uint64_t*, int, uint32_t*, float*, const uint8_t*, void*, const RulesOpts&, hipStream_t, const int* n_dev = nullptr);
@@ -1094,6 +1096,126 @@ int qz_memo_flush(qz_engine* e, void* stream) {
     }
     HIP_TRY(qzl::memo_flush(e->dev, s));
     return 0;
+}
+
+// ------------------------------------------------------------------ training operators (qz_policy.hip, qz_ortho.hip)
+static int policy_rows(const qz_policy_rows* r, PolicyRows* out) {
+    if (!r) return fail(QZ_E_INVALID, "null rows");
+    if (r->n < 0 || r->n > 0x7fffffffLL) return fail(QZ_E_INVALID, "n = %lld is not in 0 .. 2^31 - 1", (long long)r->n);
+    if (r->n_actions < 1) return fail(QZ_E_INVALID, "n_actions = %d < 1", r->n_actions);
+    if (r->dtype < QZ_F32 || r->dtype > QZ_F16) return fail(QZ_E_INVALID, "unknown element type %d", r->dtype);
+    if (r->legal_kind < QZ_LEGAL_ALL || r->legal_kind > QZ_LEGAL_BYTES) return fail(QZ_E_INVALID, "unknown legal_kind %d", r->legal_kind);
+    if (r->n > 0 && (!r->logits || !r->actions || (r->legal_kind != QZ_LEGAL_ALL && !r->legal))) return fail(QZ_E_INVALID, "null logits, actions or legal set");
+    if (r->n > 1 && r->ld < 0) return fail(QZ_E_INVALID, "negative row stride");
+    if (r->legal_kind == QZ_LEGAL_BITS && r->legal_ld < 0) return fail(QZ_E_INVALID, "negative row stride of the legal set");
+    *out = PolicyRows{r->logits, r->ld, r->n, r->actions, r->legal, r->legal_ld, r->legal_kind, r->dtype, r->n_actions};
+    return 0;
+}
+static int policy_terms(const qz_policy_rows* r, const qz_policy_terms* t, PolicyTerms* out) {
+    if (!t) return fail(QZ_E_INVALID, "null terms");
+    if (r->n > 0 && (!t->advantages || !t->old_logp)) return fail(QZ_E_INVALID, "null advantages or old_logp");
+    if (t->ref_logits && t->ref_logp) return fail(QZ_E_INVALID, "ref_logits and ref_logp exclude each other");
+    if (!(t->clip_low >= 0.f) || !(t->clip_low <= 1.f) || !(t->clip_high >= 0.f)) return fail(QZ_E_INVALID, "clip range [1 - %g, 1 + %g]", t->clip_low, t->clip_high);
+    *out = PolicyTerms{t->advantages, t->old_logp, t->ref_logp, t->weights, t->ref_logits, t->ref_ld, t->clip_low, t->clip_high, t->kl_coef, t->entropy_coef,
+                       r->n > 0 ? 1.f / (float)r->n : 0.f};
+    return 0;
+}
+static int policy_ws(const PolicyRows& R, const void* ws, int64_t bytes) {
+    const int64_t need = qzl::policy_workspace_bytes(R.n, R.a);
+    if (need > 0 && (!ws || bytes < need)) return fail(QZ_E_INVALID, "workspace of %lld bytes, %lld are needed", (long long)bytes, (long long)need);
+    return 0;
+}
+int64_t qz_policy_workspace(int64_t n, int n_actions) { return n < 0 || n_actions < 1 ? 0 : qzl::policy_workspace_bytes(n, n_actions); }
+int qz_action_logp(const qz_policy_rows* rows, float* logp, float* entropy, float* stats, void* workspace, int64_t workspace_bytes, void* stream) {
+    int r;
+    PolicyRows R;
+    if ((r = policy_rows(rows, &R)) || (r = policy_ws(R, workspace, workspace_bytes)) || (r = device_check())) return r;
+    if (R.n > 0 && !logp) return fail(QZ_E_INVALID, "null logp");
+    HIP_TRY(qzl::action_logp(R, logp, entropy, stats, workspace, (hipStream_t)stream));
+    return 0;
+}
+int qz_action_logp_backward(const qz_policy_rows* rows, const float* stats, const float* entropy, const float* dlogp, const float* dentropy, void* grad,
+                            int64_t ld_grad, void* stream) {
+    int r;
+    PolicyRows R;
+    if ((r = policy_rows(rows, &R)) || (r = device_check())) return r;
+    if (R.n > 0 && (!stats || !grad || (dentropy && !entropy))) return fail(QZ_E_INVALID, "null stats, entropy or grad");
+    if (R.n > 1 && ld_grad < R.a) return fail(QZ_E_INVALID, "gradient rows overlap: ld_grad = %lld < %d", (long long)ld_grad, R.a);
+    HIP_TRY(qzl::action_logp_backward(R, stats, entropy, dlogp, dentropy, grad, ld_grad, (hipStream_t)stream));
+    return 0;
+}
+int qz_policy_loss(const qz_policy_rows* rows, const qz_policy_terms* terms, float* loss, float* logp, float* kl, float* entropy, void* grad, int64_t ld_grad,
+                   void* workspace, int64_t workspace_bytes, void* stream) {
+    int r;
+    PolicyRows R;
+    PolicyTerms P;
+    if ((r = policy_rows(rows, &R)) || (r = policy_terms(rows, terms, &P)) || (r = policy_ws(R, workspace, workspace_bytes)) || (r = device_check())) return r;
+    if (!loss || (R.n > 0 && (!logp || !kl || !entropy))) return fail(QZ_E_INVALID, "null loss, logp, kl or entropy");
+    if (grad && R.n > 1 && ld_grad < R.a) return fail(QZ_E_INVALID, "gradient rows overlap: ld_grad = %lld < %d", (long long)ld_grad, R.a);
+    HIP_TRY(qzl::policy_loss(R, P, PolicyOut{logp, kl, entropy, grad, ld_grad, nullptr, 0, nullptr}, loss, workspace, (hipStream_t)stream));
+    return 0;
+}
+int qz_policy_loss_backward(const qz_policy_rows* rows, const qz_policy_terms* terms, const float* upstream, int only_if_scaled, void* grad, int64_t ld_grad,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+    int r;
+    PolicyRows R;
+    PolicyTerms P;
+    if ((r = policy_rows(rows, &R)) || (r = policy_terms(rows, terms, &P)) || (r = policy_ws(R, workspace, workspace_bytes)) || (r = device_check())) return r;
+    if (!upstream || (R.n > 0 && !grad)) return fail(QZ_E_INVALID, "null upstream or grad");
+    if (R.n > 1 && ld_grad < R.a) return fail(QZ_E_INVALID, "gradient rows overlap: ld_grad = %lld < %d", (long long)ld_grad, R.a);
+    HIP_TRY(qzl::policy_loss(R, P, PolicyOut{nullptr, nullptr, nullptr, grad, ld_grad, upstream, only_if_scaled, nullptr}, nullptr, workspace, (hipStream_t)stream));
+    return 0;
+}
+
+// the list as the kernels' host side takes it; `muon` = the optimiser step's pointers are checked
+static int matrix_list(const qz_matrix* list, int count, int dtype, bool muon, std::vector<OrthoMatrix>* out) {
+    if (count < 0 || (count > 0 && !list)) return fail(QZ_E_INVALID, "bad matrix list");
+    if (dtype < QZ_F32 || dtype > QZ_F16) return fail(QZ_E_INVALID, "unknown element type %d", dtype);
+    out->reserve((size_t)count);
+    for (int i = 0; i < count; i++) {
+        const qz_matrix& q = list[i];
+        const int64_t top = 1 << 20;
+        if (q.rows < 0 || q.cols < 0 || q.rows > top || q.cols > top || q.rows * q.cols > (1LL << 32))
+            return fail(QZ_E_INVALID, "matrix %d: %lld x %lld is out of range", i, (long long)q.rows, (long long)q.cols);
+        if (q.rows > 0 && q.cols > 0) {
+            if (!q.update || q.ld < 0) return fail(QZ_E_INVALID, "matrix %d: null update or negative stride", i);
+            if (muon ? (!q.momentum || !q.param) : (!q.out || (q.rows > 1 && q.out_ld < q.cols)))
+                return fail(QZ_E_INVALID, "matrix %d: null output, momentum or weight, or overlapping output rows", i);
+        }
+        out->push_back(OrthoMatrix{q.rows, q.cols, q.update, q.ld, q.out, q.out_ld, q.momentum, q.param, q.scale});
+    }
+    return 0;
+}
+static int run_matrices(const qz_matrix* list, int count, const OrthoStep& o, void* ws, int64_t ws_bytes, void* stream) {
+    try {  // (the list's copy allocates)
+        std::vector<OrthoMatrix> q;
+        int r;
+        if ((r = matrix_list(list, count, o.dtype, o.muon != 0, &q)) || (r = device_check())) return r;
+        if (o.steps < 1 || o.steps > 16) return fail(QZ_E_INVALID, "steps = %d is not in 1 .. 16", o.steps);
+        const int64_t need = qzl::ortho_workspace_bytes(q.data(), count, o);
+        if (need > 0 && (!ws || ws_bytes < need || ((uintptr_t)ws & 255))) return fail(QZ_E_INVALID, "workspace of %lld bytes, %lld are needed, 256-byte aligned", (long long)ws_bytes, (long long)need);
+        HIP_TRY(qzl::orthogonalize(q.data(), count, o, ws, (hipStream_t)stream));
+        return 0;
+    } catch (const std::bad_alloc&) {
+        return fail(QZ_E_OOM, "out of host memory");
+    }
+}
+int64_t qz_orthogonalize_workspace(const qz_matrix* list, int count) {
+    if (count <= 0 || !list) return 0;
+    int64_t n = 0;
+    for (int i = 0; i < count; i++) {
+        const OrthoMatrix q = {list[i].rows, list[i].cols, nullptr, 0, nullptr, 0, nullptr, nullptr, 0.f};
+        n += qzl::ortho_workspace_bytes(&q, 1, OrthoStep{});
+    }
+    return n;
+}
+int qz_orthogonalize(const qz_matrix* list, int count, int dtype, int steps, void* workspace, int64_t workspace_bytes, void* stream) {
+    return run_matrices(list, count, OrthoStep{dtype, steps, 0, 0, 0.f, 0.f, 0.f, nullptr}, workspace, workspace_bytes, stream);
+}
+int qz_muon_step(const qz_matrix* list, int count, int dtype, int steps, const qz_muon_opts* opts, void* workspace, int64_t workspace_bytes, void* stream) {
+    if (!opts) return fail(QZ_E_INVALID, "null options");
+    return run_matrices(list, count, OrthoStep{dtype, steps, 1, opts->nesterov, opts->lr, opts->momentum, opts->weight_decay, opts->lr_dev}, workspace,
+                        workspace_bytes, stream);
 }
 
 // self-test hook used by the GPU tests: device sqrt(double(i)) for i in [0, n)

@@ -1,0 +1,481 @@
+// qz_policy.hip -- log-probabilities of actions and the clipped policy loss, forward and backward.
+//
+// A row is one decision: n_actions logits z, a legal set, the action a that was taken.
+//   p_j = exp(z_j - lse) over the legal columns, lse = log sum_legal exp z_j,
+//   log pi(a) = z_a - lse, taken as (z_a - m) - log s (m may be a mask's lowest value, next to which log s would vanish),
+//   H = lse - sum p_j z_j = log s - t / s with s = sum e^(z-m), t = sum e^(z-m) (z-m), m = max z
+//   (both terms of the last form are >= 0: no cancellation).
+// The loss of a row (w = its weight, A = its advantage, r = exp(log pi(a) - old)):
+//   L = w [ -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta KL - eta H ]
+//   KL over a frozen policy's logits: sum q (log q - log p), computed as sum q (e^x - 1 - x), x = log p - log q: every
+//   term is >= 0 and an error of lse cancels to first order, where the plain sum loses all digits of a small KL.
+//   KL from the frozen policy's log-probability of a alone: e^x - 1 - x with x = log q(a) - log p(a).
+//   dL/dz_j = w [ c (delta_ja - p_j) + beta (p_j - q_j) + eta p_j (log p_j + H) ],
+//   c = -A r where the ratio is not clipped, minus beta (e^x - 1) for the second form of KL.
+// A row whose action is negative, out of range, illegal or has a logit of -inf is LEFT OUT: zero loss, gradient, KL and
+// entropy.  Illegal columns are never read into arithmetic (they may hold NaN or infinities) and get a zero gradient.
+// All sums are float32 (row) and float64 (over rows), in an order fixed by the shape: results repeat bit for bit.
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qz_policy.h"
+
+#pragma clang fp contract(fast)
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log_fast(float x) { return __builtin_amdgcn_logf(x) * LN2; }
+
+// ---- elements: V of them are 16 bytes.  Rows may start at any element (odd widths): the 16-byte accesses are declared with
+// the element's alignment, which the hardware serves in one instruction.
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ float get(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+    static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
+};
+template <>
+struct Elem<__hip_bfloat16> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ float get(const void* p, int64_t i) {
+        return __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
+    }
+    static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<__bf16*>(p)[i] = (__bf16)v; }
+};
+template <>
+struct Elem<__half> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ float get(const void* p, int64_t i) { return (float)static_cast<const _Float16*>(p)[i]; }
+    static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<_Float16*>(p)[i] = (_Float16)v; }
+};
+
+struct Raw {
+    uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Raw load_chunk(const void* row, int64_t j0, int n) {
+    Raw r = {{0u, 0u, 0u, 0u}};
+    if (j0 + Elem<T>::V <= n) {
+        __builtin_memcpy(&r, static_cast<const T*>(row) + j0, 16);
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (j0 + k < n) r.w[k] = static_cast<const uint32_t*>(row)[j0 + k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (j0 + k < n) r.w[k >> 1] |= (uint32_t) static_cast<const uint16_t*>(row)[j0 + k] << (16 * (k & 1));
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float chunk_get(const Raw& r, int k);
+template <>
+__device__ __forceinline__ float chunk_get<float>(const Raw& r, int k) { return __uint_as_float(r.w[k]); }
+template <>
+__device__ __forceinline__ float chunk_get<__hip_bfloat16>(const Raw& r, int k) {
+    return __uint_as_float((k & 1) ? (r.w[k >> 1] & 0xFFFF0000u) : (r.w[k >> 1] << 16));
+}
+template <>
+__device__ __forceinline__ float chunk_get<__half>(const Raw& r, int k) {
+    const uint16_t h = (uint16_t)(r.w[k >> 1] >> (16 * (k & 1)));
+    return (float)__builtin_bit_cast(_Float16, h);
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(void* row, int64_t j0, int n, const float* v) {
+    if (j0 + Elem<T>::V <= n) {
+        Raw r;
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) r.w[k] = __float_as_uint(v[k]);
+        } else if (__is_same(T, __half)) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k + 1]) << 16;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k + 1]) << 16;
+        }
+        __builtin_memcpy(static_cast<T*>(row) + j0, &r, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < Elem<T>::V; k++)
+            if (j0 + k < n) Elem<T>::put(row, j0 + k, v[k]);
+    }
+}
+
+// ---- legal sets: bit k of the result <=> column j0 + k exists and is legal
+template <int V>
+__device__ __forceinline__ uint32_t legal_bits(const PolicyRows& R, int64_t row, int64_t j0) {
+    const int64_t left = (int64_t)R.a - j0;
+    if (left <= 0) return 0u;
+    const uint32_t inside = left >= V ? (1u << V) - 1u : (1u << (int)left) - 1u;
+    if (R.legal_kind == 0) return inside;
+    if (R.legal_kind == 1) {  // V divides 32 and j0 is a multiple of V: the bits sit in one word
+        const uint32_t w = static_cast<const uint32_t*>(R.legal)[row * R.legal_ld + (j0 >> 5)];
+        return (w >> (j0 & 31)) & inside;
+    }
+    const uint8_t* b = static_cast<const uint8_t*>(R.legal) + row * R.legal_ld + j0;
+    uint32_t m = 0u;
+    if (left >= V) {
+        uint8_t t[V];
+        __builtin_memcpy(t, b, V);
+#pragma unroll
+        for (int k = 0; k < V; k++) m |= (t[k] ? 1u : 0u) << k;
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            if (k < left) m |= (b[k] ? 1u : 0u) << k;
+    }
+    return m;
+}
+__device__ __forceinline__ bool legal_one(const PolicyRows& R, int64_t row, int64_t j) {
+    if (R.legal_kind == 0) return true;
+    if (R.legal_kind == 1) return (static_cast<const uint32_t*>(R.legal)[row * R.legal_ld + (j >> 5)] >> (j & 31)) & 1u;
+    return static_cast<const uint8_t*>(R.legal)[row * R.legal_ld + j] != 0;
+}
+
+// ---- one row's statistics
+struct Stat {
+    float m, s, t;  // max, sum e^(z-m), sum e^(z-m) (z-m)
+};
+__device__ __forceinline__ Stat stat_empty() { return {NEG_INF, 0.f, 0.f}; }
+__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
+    // an empty side has m = -inf, s = t = 0; a NaN on either side stays (its s is NaN)
+    const float m = fmaxf(a.m, b.m);
+    const float da = a.m == m ? 0.f : a.m - m, db = b.m == m ? 0.f : b.m - m;
+    const float ea = a.s == 0.f ? 0.f : exp2_fast(da * LOG2E), eb = b.s == 0.f ? 0.f : exp2_fast(db * LOG2E);
+    Stat r;
+    r.m = m;
+    r.s = a.s * ea + b.s * eb;
+    r.t = (ea != 0.f ? (a.t + a.s * da) * ea : 0.f * a.t) + (eb != 0.f ? (b.t + b.s * db) * eb : 0.f * b.t);
+    return r;
+}
+__device__ __forceinline__ float stat_log(const Stat& s) { return log_fast(s.s); }
+__device__ __forceinline__ float stat_entropy(const Stat& s) { return fmaxf(log_fast(s.s), 0.f) - s.t / s.s; }
+
+// the action's row: live = the action is in range, legal and its logit is not -inf
+template <typename T>
+__device__ __forceinline__ bool row_live(const PolicyRows& R, int64_t row, int64_t& act, float& za) {
+    act = R.actions[row];
+    za = 0.f;
+    if (act < 0 || act >= R.a || !legal_one(R, row, act)) return false;
+    za = Elem<T>::get(static_cast<const T*>(R.logits) + row * R.ld, act);
+    return za != NEG_INF;
+}
+
+struct Coef {      // what the gradient of a row needs
+    float m, ls, h, c, beta, eta, mq, lsq;  // max and log of the sum, of pi and the frozen policy; c, beta, eta carry the row's weight
+    int64_t act;
+    bool on;  // false: weight 0, no gradient whatever the row holds
+};
+struct RowOut {
+    float logp, loss;  // loss without its KL over logits
+    Coef g;
+};
+__device__ __forceinline__ float expm1_minus_x(float x) {  // e^x - 1 - x >= 0
+    if (fabsf(x) < 0.5f) {
+        float r = 1.f / 40320.f;
+        r = r * x + 1.f / 5040.f;
+        r = r * x + 1.f / 720.f;
+        r = r * x + 1.f / 120.f;
+        r = r * x + 1.f / 24.f;
+        r = r * x + 1.f / 6.f;
+        r = r * x + 0.5f;
+        return r * x * x;
+    }
+    return expf(x) - 1.f - x;
+}
+__device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, int64_t act, float za, const Stat& st, const Stat& sq, float scale) {
+    RowOut o;
+    const float h = stat_entropy(st);
+    o.g.m = st.m;
+    o.g.ls = stat_log(st);
+    o.g.mq = sq.m;
+    o.g.lsq = stat_log(sq);
+    o.logp = (za - o.g.m) - o.g.ls;
+    const float w = P.weights ? P.weights[row] : P.default_weight;
+    const float adv = P.advantages[row], r = expf(o.logp - P.old_logp[row]);
+    const float open = r * adv, held = fminf(fmaxf(r, 1.f - P.clip_low), 1.f + P.clip_high) * adv;
+    // a NaN ratio or advantage must reach the loss and the gradient: the comparisons are written so that it takes their first branch
+    const bool held_wins = held < open;
+    float c = held_wins ? 0.f : -open;
+    o.loss = held_wins ? -held : -open;
+    if (P.ref_logp) {
+        const float x = P.ref_logp[row] - o.logp, f = expm1_minus_x(x);
+        o.loss += P.kl_coef * f;
+        c -= P.kl_coef * (f + x);
+    }
+    o.loss -= P.entropy_coef * h;
+    const bool on = w != 0.f;
+    o.loss = on ? w * o.loss : 0.f;
+    const float ws = w * scale;
+    o.g.h = h;
+    o.g.c = on ? ws * c : 0.f;
+    o.g.beta = on && P.ref_logits ? ws * P.kl_coef : 0.f;
+    o.g.eta = on ? ws * P.entropy_coef : 0.f;
+    o.g.act = act;
+    o.g.on = on;
+    return o;
+}
+__device__ __forceinline__ float kl_taken(const PolicyTerms& P, int64_t row, float logp) { return P.ref_logp ? expm1_minus_x(P.ref_logp[row] - logp) : 0.f; }
+
+// one column: gradient, and the column's term of KL over logits.  p = 0 (a logit of -inf) gives 0 log 0 = 0; q = 0 < p has no KL
+// term but p; q > 0 = p is an infinite KL, as it should be.
+__device__ __forceinline__ float column(const Coef& g, bool has_q, float z, float zq, int64_t j, float& kl) {
+    const float dz = z - g.m, lp = dz - g.ls;
+    const float p = exp2_fast(lp * LOG2E);
+    float d = p * (g.eta * ((p > 0.f || lp != lp ? lp : 0.f) + g.h) - g.c);
+    if (has_q) {
+        const float dq = zq - g.mq, lq = dq - g.lsq, q = exp2_fast(lq * LOG2E);
+        const float x = (dz - dq) - (g.ls - g.lsq);
+        float f;
+        if (fabsf(x) < 0.25f) {  // p and q agree to within 25 %: their difference from the series, not from p - q
+            float r = 1.f / 720.f;
+            r = r * x + 1.f / 120.f;
+            r = r * x + 1.f / 24.f;
+            r = r * x + 1.f / 6.f;
+            r = r * x + 0.5f;
+            f = q * (r * x * x);
+        } else {
+            f = q == 0.f ? p : (p - q) - q * x;
+        }
+        kl += f;
+        d += g.beta * (p - q);
+    }
+    if (j == g.act) d += g.c;
+    return g.on ? d : 0.f;
+}
+
+// ---- reductions
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float v, F f) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = f(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    return wave_reduce(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ Stat wave_join(Stat s) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        Stat b = {__shfl_xor(s.m, o), __shfl_xor(s.s, o), __shfl_xor(s.t, o)};
+        // both lanes of a pair join in the same order, so that all lanes end with the same bits
+        s = (threadIdx.x & o) ? stat_join(b, s) : stat_join(s, b);
+    }
+    return s;
+}
+template <int NT>
+__device__ __forceinline__ Stat block_join(Stat s, float* sh /*[3 * NT / 64]*/) {
+    s = wave_join(s);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        sh[3 * wave] = s.m;
+        sh[3 * wave + 1] = s.s;
+        sh[3 * wave + 2] = s.t;
+    }
+    __syncthreads();
+    Stat r = {sh[0], sh[1], sh[2]};
+    for (int w = 1; w < NT / 64; w++) r = stat_join(r, Stat{sh[3 * w], sh[3 * w + 1], sh[3 * w + 2]});
+    __syncthreads();
+    return r;
+}
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* sh) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = sh[0];
+    for (int w = 1; w < NT / 64; w++) r += sh[w];
+    __syncthreads();
+    return r;
+}
+
+// the statistics of the columns that one thread visits, online: one running (m, s, t), rescaled once per 16-byte chunk
+template <typename T>
+__device__ __forceinline__ void stat_chunk(Stat& st, const Raw& raw, uint32_t ok) {
+    constexpr int V = Elem<T>::V;
+    float cm = NEG_INF;
+    bool bad = false;
+#pragma unroll
+    for (int k = 0; k < V; k++)
+        if ((ok >> k) & 1u) {
+            const float z = chunk_get<T>(raw, k);
+            cm = fmaxf(cm, z);
+            bad |= z != z;
+        }
+    if (bad) st.s = __builtin_nanf("");
+    if (cm > st.m) {
+        const float d = st.m - cm, e = st.s == 0.f ? 0.f : exp2_fast(d * LOG2E);
+        st.t = e != 0.f ? (st.t + st.s * d) * e : 0.f;
+        st.s = st.s != st.s ? st.s : st.s * e;
+        st.m = cm;
+    }
+    if (st.m == NEG_INF) return;
+#pragma unroll
+    for (int k = 0; k < V; k++)
+        if ((ok >> k) & 1u) {
+            const float x = chunk_get<T>(raw, k) - st.m, e = exp2_fast(x * LOG2E);
+            st.s += e;
+            st.t += e != 0.f ? e * x : 0.f;
+        }
+}
+
+// ================================================================ any width: one workgroup per row, the row read twice
+constexpr int RT = 256;
+
+template <typename T>
+__device__ __forceinline__ Stat row_stat(const PolicyRows& R, const void* base, int64_t ld, int64_t row, float* sh) {
+    const T* z = static_cast<const T*>(base) + row * ld;
+    Stat st = stat_empty();
+    for (int64_t j = (int64_t)threadIdx.x * Elem<T>::V; j < R.a; j += RT * Elem<T>::V) stat_chunk<T>(st, load_chunk<T>(z, j, R.a), legal_bits<Elem<T>::V>(R, row, j));
+    return block_join<RT>(st, sh);
+}
+
+template <typename T>
+__global__ __launch_bounds__(RT) void k_action_logp(PolicyRows R, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
+    __shared__ float sh[3 * RT / 64];
+    const int64_t row = blockIdx.x;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    Stat st = stat_empty();
+    if (live) st = row_stat<T>(R, R.logits, R.ld, row, sh);
+    if (threadIdx.x == 0) {
+        const float ls = stat_log(st);
+        logp[row] = live ? (za - st.m) - ls : act < 0 ? 0.f : NEG_INF;
+        if (entropy) entropy[row] = live ? stat_entropy(st) : 0.f;
+        if (stats) {
+            stats[row] = live ? st.m : 0.f;
+            stats[R.n + row] = live ? ls : 0.f;
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(RT) void k_action_logp_backward(PolicyRows R, const float* __restrict__ stats, const float* __restrict__ entropy,
+                                                             const float* __restrict__ dlogp, const float* __restrict__ dentropy, void* __restrict__ grad,
+                                                             int64_t ld_grad) {
+    constexpr int V = Elem<T>::V;
+    const int64_t row = blockIdx.x;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    const T* z = static_cast<const T*>(R.logits) + row * R.ld;
+    T* out = static_cast<T*>(grad) + row * ld_grad;
+    const Coef g = {stats[row], stats[R.n + row], entropy ? entropy[row] : 0.f, dlogp ? dlogp[row] : 0.f, 0.f, dentropy ? -dentropy[row] : 0.f, 0.f, 0.f, act, true};
+    for (int64_t j = ((int64_t)blockIdx.y * RT + threadIdx.x) * V; j < R.a; j += (int64_t)gridDim.y * RT * V) {
+        const uint32_t ok = live ? legal_bits<V>(R, row, j) : 0u;
+        const Raw raw = load_chunk<T>(z, j, R.a);
+        float d[V], kl = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; k++) d[k] = (ok >> k) & 1u ? column(g, false, chunk_get<T>(raw, k), 0.f, j + k, kl) : 0.f;
+        store_chunk<T>(out, j, R.a, d);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P, PolicyOut O) {
+    constexpr int V = Elem<T>::V;
+    __shared__ float sh[3 * RT / 64];
+    const float scale = O.scale ? *O.scale : 1.f;
+    if (O.only_if_scaled && scale == 1.f) return;  // the gradient that the forward pass wrote is the one asked for
+    const int64_t row = blockIdx.x;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    T* out = static_cast<T*>(O.grad) + row * O.ld_grad;
+    float kl = 0.f;
+    RowOut o = {act < 0 ? 0.f : NEG_INF, 0.f, {}};
+    float h = 0.f;
+    if (live) {
+        const Stat st = row_stat<T>(R, R.logits, R.ld, row, sh);
+        const bool has_q = P.ref_logits != nullptr;
+        const Stat sq = has_q ? row_stat<T>(R, P.ref_logits, P.ref_ld, row, sh) : Stat{0.f, 1.f, 0.f};
+        h = stat_entropy(st);
+        o = row_terms(P, row, act, za, st, sq, scale);
+        const T* z = static_cast<const T*>(R.logits) + row * R.ld;
+        const T* zq = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
+        if (O.grad || has_q) {
+            for (int64_t j = (int64_t)threadIdx.x * V; j < R.a; j += RT * V) {
+                const uint32_t ok = legal_bits<V>(R, row, j);
+                const Raw raw = load_chunk<T>(z, j, R.a);
+                Raw rq = {};
+                if (has_q) rq = load_chunk<T>(zq, j, R.a);
+                float d[V];
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    d[k] = (ok >> k) & 1u ? column(o.g, has_q, chunk_get<T>(raw, k), has_q ? chunk_get<T>(rq, k) : 0.f, j + k, kl) : 0.f;
+                if (O.grad) store_chunk<T>(out, j, R.a, d);
+            }
+        }
+        kl = has_q ? block_sum<RT>(kl, sh) : kl_taken(P, row, o.logp);
+    } else if (O.grad) {
+        const float zero[V] = {};
+        for (int64_t j = (int64_t)threadIdx.x * V; j < R.a; j += RT * V) store_chunk<T>(out, j, R.a, zero);
+    }
+    if (threadIdx.x == 0 && O.parts) {
+        const float w = P.weights ? P.weights[row] : P.default_weight;
+        O.logp[row] = o.logp;
+        O.kl[row] = live ? kl : 0.f;
+        O.entropy[row] = h;
+        O.parts[row] = (double)o.loss + (P.ref_logits && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+    }
+}
+
+__global__ __launch_bounds__(1024) void k_sum_parts(const double* __restrict__ parts, int64_t n, float* __restrict__ loss) {
+    __shared__ double sh[1024];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += parts[i];
+    sh[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 512; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = (float)sh[0];
+}
+
+}  // namespace
+
+#define BY_TYPE(dtype, CALL)                                                              \
+    switch (dtype) {                                                                      \
+        case 0: { using T = float; CALL; break; }                                         \
+        case 1: { using T = __hip_bfloat16; CALL; break; }                                \
+        default: { using T = __half; CALL; break; }                                       \
+    }
+
+namespace qzl {
+int64_t policy_workspace_bytes(int64_t n, int a) { return n * (int64_t)sizeof(double); }
+
+hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void*, hipStream_t s) {
+    if (R.n <= 0) return hipSuccess;
+    BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, logp, entropy, stats));
+    return hipGetLastError();
+}
+hipError_t action_logp_backward(const PolicyRows& R, const float* stats, const float* entropy, const float* dlogp, const float* dentropy, void* grad,
+                                int64_t ld_grad, hipStream_t s) {
+    if (R.n <= 0) return hipSuccess;
+    BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp_backward<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, stats, entropy, dlogp, dentropy, grad, ld_grad));
+    return hipGetLastError();
+}
+hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, float* loss, void* ws, hipStream_t s) {
+    O.parts = loss ? static_cast<double*>(ws) : nullptr;
+    if (R.n > 0) BY_TYPE(R.dtype, hipLaunchKernelGGL((k_policy_loss<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, P, O));
+    if (loss) hipLaunchKernelGGL(k_sum_parts, dim3(1), dim3(1024), 0, s, O.parts, R.n, loss);
+    return hipGetLastError();
+}
+}  // namespace qzl

@@ -1,0 +1,285 @@
+"""Policy losses on the GPU: log-probabilities of actions under a legal-move mask, and the clipped policy loss with its KL and
+entropy terms, each with its gradient (csrc/qz_policy.hip through the C ABI: qz_action_logp, qz_policy_loss).
+
+``logits`` are [..., A]: any number of decisions over A actions (float32, bfloat16 or float16; log-probabilities serve as
+logits too).  ``legal`` is None, a mask of bytes or bools [..., A], or packed 32-bit words [..., ceil(A / 32)] -- what
+``rules.movegen`` returns.  Its leading dimensions broadcast.  A decision whose action is negative, out of range, illegal or
+has a logit of -inf is left out: no loss, no gradient, no entropy; its log-probability reads 0 for a negative action (padding)
+and -inf otherwise.  Illegal columns may hold anything, NaN included.
+
+There is no CPU path: tensors on another device than a GPU raise ``QzError(QZ_E_NO_DEVICE)``."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _cabi
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_BITS = (torch.int32, torch.uint32)
+_BYTES = (torch.bool, torch.uint8)
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor     # scalar float32, the only differentiable member
+    logp: torch.Tensor     # log pi(a), float32, one per decision; the same for the others
+    kl: torch.Tensor       # KL term of every decision (0 without a frozen policy)
+    entropy: torch.Tensor
+
+
+def _gpu(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a tensor" % name)
+    if not t.is_cuda:
+        raise _cabi.QzError(_cabi.E_NO_DEVICE, "%s is on %s; this package has no CPU path" % (name, t.device))
+
+
+def _same_device(t, device, name):
+    _gpu(t, name)
+    if t.device != device:
+        raise ValueError("%s is on %s, the logits on %s" % (name, t.device, device))
+
+
+def _rows_of(logits, name="logits"):
+    """[..., A] -> [n, A] whose rows are contiguous (a view wherever there is one)."""
+    _gpu(logits, name)
+    if logits.dtype not in DTYPES:
+        raise TypeError("%s: %s is not one of float32, bfloat16, float16" % (name, logits.dtype))
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("%s: at least one action is needed, got the shape %s" % (name, tuple(logits.shape)))
+    return logits.reshape(-1, logits.shape[-1])
+
+
+def _unit_rows(t):
+    # (a row stride below the row's length is fine for an input: broadcast rows)
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _vector(t, lead, device, name):
+    """A float per decision, constant for the gradient."""
+    if t is None:
+        return None
+    _same_device(t, device, name)
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires grad, but the loss treats it as a constant: detach it" % name)
+    if not t.is_floating_point():
+        raise TypeError("%s must be floating point" % name)
+    if tuple(t.shape) != tuple(lead):
+        raise ValueError("%s has the shape %s, %s is needed" % (name, tuple(t.shape), tuple(lead)))
+    return t.to(torch.float32).reshape(-1).contiguous()
+
+
+def _actions(t, lead, device):
+    _same_device(t, device, "actions")
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError("actions must be integers")
+    if tuple(t.shape) != tuple(lead):
+        raise ValueError("actions have the shape %s, %s is needed" % (tuple(t.shape), tuple(lead)))
+    return t.to(torch.int64).reshape(-1).contiguous()
+
+
+def _legal(t, lead, a, device):
+    """-> (tensor [n, words or bytes] or None, kind)"""
+    if t is None:
+        return None, 0
+    _same_device(t, device, "legal")
+    kind, width = (1, (a + 31) // 32) if t.dtype in _BITS else (2, a) if t.dtype in _BYTES else (0, 0)
+    if not kind:
+        raise TypeError("legal: %s is neither packed 32-bit words nor bytes" % t.dtype)
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError("legal has the shape %s, its last dimension must be %d" % (tuple(t.shape), width))
+    return _unit_rows(t.expand(tuple(lead) + (width,)).reshape(-1, width)), kind
+
+
+def _struct(z, actions, legal, kind):
+    return _cabi.qz_policy_rows(z.data_ptr(), z.stride(0), z.shape[0], z.shape[1], DTYPES[z.dtype], actions.data_ptr(),
+                                legal.data_ptr() if kind else 0, legal.stride(0) if kind else 0, kind)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else 0
+
+
+def _workspace(n, a, device):
+    size = _cabi.load().qz_policy_workspace(n, a)
+    return torch.empty(max(size, 1), dtype=torch.uint8, device=device), size
+
+
+class _Launch:
+    """The tensor's device made current (only if it is not), and its current stream."""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if torch.cuda.current_device() != device.index else None
+        self.device = device
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _refuse_captured_leaf(logits):
+    # the backward pass of a leaf runs on the stream that the leaf's gradient was first accumulated on: inside a capture that
+    # may be a stream outside of it, which ends the process
+    if logits.is_leaf and logits.requires_grad and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("logits that are leaves cannot be differentiated inside a graph capture: use policy_loss_and_grad, or let "
+                           "the network that makes them run inside the capture too")
+
+
+class _ActionLogp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, actions, legal, kind, want_entropy):
+        n, a = z.shape
+        z = _unit_rows(z)
+        logp = torch.empty(n, dtype=torch.float32, device=z.device)
+        need = ctx.needs_input_grad[0]
+        entropy = torch.empty_like(logp) if want_entropy else None
+        stats = torch.empty((2, n), dtype=torch.float32, device=z.device) if need else None
+        ws, size = _workspace(n, a, z.device)
+        with _Launch(z.device) as stream:
+            _cabi.check(_cabi.load().qz_action_logp(C.byref(_struct(z, actions, legal, kind)), logp.data_ptr(), _ptr(entropy), _ptr(stats), ws.data_ptr(),
+                                                    size, stream))
+        ctx.kind = kind
+        ctx.save_for_backward(z, actions, legal, stats, entropy)
+        ctx.set_materialize_grads(False)
+        return (logp, entropy) if want_entropy else logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp, dentropy=None):
+        z, actions, legal, stats, entropy = ctx.saved_tensors
+        if dlogp is None and dentropy is None:
+            return None, None, None, None, None
+        dlogp = dlogp.contiguous() if dlogp is not None else None
+        dentropy = dentropy.contiguous() if dentropy is not None else None
+        grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        with _Launch(z.device) as stream:
+            _cabi.check(_cabi.load().qz_action_logp_backward(C.byref(_struct(z, actions, legal, ctx.kind)), stats.data_ptr(), _ptr(entropy), _ptr(dlogp),
+                                                             _ptr(dentropy), grad.data_ptr(), grad.stride(0), stream))
+        return grad, None, None, None, None
+
+
+def action_logp(logits, actions, legal=None, entropy=False):
+    """log pi(action) of every decision, float32 with the shape of ``actions``; with ``entropy=True`` a pair of that and the
+    entropy of the distribution over the legal actions.  Differentiable in ``logits``."""
+    lead = tuple(logits.shape[:-1]) if isinstance(logits, torch.Tensor) else ()
+    z = _rows_of(logits)
+    _refuse_captured_leaf(logits)
+    acts = _actions(actions, lead, z.device)
+    mask, kind = _legal(legal, lead, z.shape[1], z.device)
+    out = _ActionLogp.apply(z, acts, mask, kind, bool(entropy))
+    if entropy:
+        return out[0].reshape(lead), out[1].reshape(lead)
+    return out.reshape(lead)
+
+
+class _Terms(NamedTuple):
+    clip_low: float
+    clip_high: float
+    kl_coef: float
+    entropy_coef: float
+    kind: int
+
+    def struct(self, advantages, old_logp, ref_logp, weights, ref):
+        return _cabi.qz_policy_terms(advantages.data_ptr(), old_logp.data_ptr(), _ptr(ref_logp), _ptr(weights), _ptr(ref),
+                                     ref.stride(0) if ref is not None else 0, self.clip_low, self.clip_high, self.kl_coef, self.entropy_coef)
+
+
+def _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, want_grad):
+    n, a = z.shape
+    row = torch.empty((3, n), dtype=torch.float32, device=z.device)
+    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    grad = torch.empty((n, a), dtype=z.dtype, device=z.device) if want_grad else None
+    ws, size = _workspace(n, a, z.device)
+    t = terms.struct(advantages, old_logp, ref_logp, weights, ref)
+    with _Launch(z.device) as stream:
+        _cabi.check(_cabi.load().qz_policy_loss(C.byref(_struct(z, actions, legal, terms.kind)), C.byref(t), loss.data_ptr(), row[0].data_ptr(),
+                                                row[1].data_ptr(), row[2].data_ptr(), _ptr(grad), a, ws.data_ptr(), size, stream))
+    return loss, row[0], row[1], row[2], grad
+
+
+class _ClippedPolicyLoss(torch.autograd.Function):
+    """The forward pass writes the gradient for an upstream factor of 1 beside the loss (one pass over the logits for both);
+    the backward pass hands it out, or computes it again where the factor is another or it was handed out before."""
+
+    @staticmethod
+    def forward(ctx, z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms):
+        z = _unit_rows(z)
+        loss, logp, kl, entropy, grad = _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, ctx.needs_input_grad[0])
+        ctx.terms, ctx.grad = terms, grad
+        ctx.save_for_backward(z, actions, legal, advantages, old_logp, ref_logp, weights, ref)
+        ctx.mark_non_differentiable(logp, kl, entropy)
+        return loss, logp, kl, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream, *_):
+        z, actions, legal, advantages, old_logp, ref_logp, weights, ref = ctx.saved_tensors
+        grad, ctx.grad = ctx.grad, None
+        fresh = grad is None
+        if fresh:
+            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        ws, size = _workspace(z.shape[0], z.shape[1], z.device)
+        t = ctx.terms.struct(advantages, old_logp, ref_logp, weights, ref)
+        upstream = upstream.contiguous()
+        with _Launch(z.device) as stream:
+            _cabi.check(_cabi.load().qz_policy_loss_backward(C.byref(_struct(z, actions, legal, ctx.terms.kind)), C.byref(t), upstream.data_ptr(),
+                                                             0 if fresh else 1, grad.data_ptr(), grad.stride(0), ws.data_ptr(), size, stream))
+        return (grad,) + (None,) * 8
+
+
+def _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef):
+    z = _rows_of(logits)
+    lead, device = tuple(logits.shape[:-1]), z.device
+    low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+    low, high = float(low), float(high)
+    if not (0.0 <= low <= 1.0 and high >= 0.0):
+        raise ValueError("clip = %r: the ratio's range is [1 - low, 1 + high] with 0 <= low <= 1 and high >= 0" % (clip,))
+    if ref_logits is not None and ref_logp is not None:
+        raise ValueError("ref_logits and ref_logp exclude each other")
+    ref = None
+    if ref_logits is not None:
+        _same_device(ref_logits, device, "ref_logits")
+        if ref_logits.requires_grad and torch.is_grad_enabled():
+            raise ValueError("ref_logits require grad, but the loss treats them as constants: detach them")
+        if ref_logits.shape != logits.shape or ref_logits.dtype != logits.dtype:
+            raise ValueError("ref_logits: %s %s, the logits are %s %s" % (tuple(ref_logits.shape), ref_logits.dtype, tuple(logits.shape), logits.dtype))
+        ref = _unit_rows(_rows_of(ref_logits, "ref_logits"))
+    if advantages is None or old_logp is None:
+        raise TypeError("advantages and old_logp are needed")
+    mask, kind = _legal(legal, lead, z.shape[1], device)
+    terms = _Terms(low, high, float(kl_coef), float(entropy_coef), kind)
+    return (z, _actions(actions, lead, device), mask, _vector(advantages, lead, device, "advantages"), _vector(old_logp, lead, device, "old_logp"),
+            _vector(ref_logp, lead, device, "ref_logp"), _vector(weights, lead, device, "weights"), ref, terms), lead
+
+
+def clipped_policy_loss(logits, actions, advantages, old_logp, legal: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                        ref_logits: Optional[torch.Tensor] = None, ref_logp: Optional[torch.Tensor] = None, clip=0.2, kl_coef=0.0,
+                        entropy_coef=0.0) -> PolicyLoss:
+    """sum_i w_i [ -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef KL - entropy_coef H ] with r = exp(log pi(a) - old_logp).
+
+    weights: w_i (default 1 / n each; 0 leaves a decision out of the loss).  clip: one number, or (low, high).
+    KL(frozen || pi) over ref_logits (same shape and type as the logits), or estimated from ref_logp, the frozen policy's
+    log-probability of the action, as e^x - 1 - x with x = ref_logp - log pi(a).
+    Differentiable in ``logits``; memory for their gradient is taken in the forward pass."""
+    args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
+    _refuse_captured_leaf(logits)
+    loss, logp, kl, entropy = _ClippedPolicyLoss.apply(*args)
+    return PolicyLoss(loss, logp.reshape(lead), kl.reshape(lead), entropy.reshape(lead))
+
+
+@torch.no_grad()
+def policy_loss_and_grad(logits, actions, advantages, old_logp, legal=None, weights=None, ref_logits=None, ref_logp=None, clip=0.2, kl_coef=0.0,
+                         entropy_coef=0.0):
+    """(PolicyLoss, gradient of its loss in the logits) without the autograd graph: what a captured HIP graph records."""
+    args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
+    z = _unit_rows(args[0])
+    loss, logp, kl, entropy, grad = _run_loss(z, *args[1:], True)
+    return PolicyLoss(loss, logp.reshape(lead), kl.reshape(lead), entropy.reshape(lead)), grad.reshape(logits.shape)

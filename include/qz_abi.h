@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define QZ_ABI_VERSION 7
+#define QZ_ABI_VERSION 8
 #define QZ_N_ACTIONS 140            /* quoridor.py:12  action_space = 140            */
 #define QZ_PLANES (26 * 81)         /* quoridor.py:58-131  26x9x9 state tensor       */
 #define QZ_MASK_WORDS 5             /* 140-bit legal mask, bit a of word a/32        */
@@ -472,6 +472,89 @@ int qz_selfplay_misses(qz_engine* e, qz_boards* boards_out, const int32_t** n_de
 /* the weights changed (training step, checkpoint load): every stored evaluation is dead.  O(1): bumps the epoch the
  * memo's keys carry. */
 int qz_memo_flush(qz_engine* e, void* stream);
+
+/* ------------------------------------------------------------- training operators
+ * What policy_update / train_step (train.py:65-92, policy_value_net.py:166-192) need beyond the network itself: the
+ * log-probability of the action taken under the legal-move mask, the clipped policy loss with its KL and entropy terms and its
+ * gradient, and the optimiser step with orthogonalised updates (csrc/qz_policy.hip, csrc/qz_ortho.hip: the formulas).  Element
+ * types: QZ_F32 | QZ_BF16 | QZ_F16.  Workspaces are the caller's (device memory, 256-byte aligned) and hold nothing between
+ * calls: calls that may run at the same time, and captured graphs that may, each need one of their own. */
+#define QZ_F32 0
+#define QZ_BF16 1
+#define QZ_F16 2
+#define QZ_LEGAL_ALL 0
+#define QZ_LEGAL_BITS 1             /* uint32 words, bit j % 32 of word j / 32 (the layout of mask5)   */
+#define QZ_LEGAL_BYTES 2            /* one byte per column, non-zero = legal                           */
+/* n decisions over n_actions columns.  A row is LEFT OUT (zero loss, gradient, KL, entropy; log-probability 0 if its action is
+ * negative, else -inf) if its action is negative, >= n_actions, illegal, or has a logit of -inf.  What illegal columns hold is
+ * never used (NaN and infinities may stand there); their gradient is zero. */
+typedef struct {
+    const void* logits;             /* [dev] n rows of n_actions elements                              */
+    int64_t ld;                     /* elements between rows                                           */
+    int64_t n;
+    int32_t n_actions;
+    int32_t dtype;
+    const int64_t* actions;         /* [dev][n]                                                        */
+    const void* legal;              /* [dev] or NULL                                                   */
+    int64_t legal_ld;               /* words / bytes between rows                                      */
+    int32_t legal_kind;             /* QZ_LEGAL_*                                                      */
+} qz_policy_rows;
+typedef struct {
+    const float* advantages;        /* [dev][n]                                                        */
+    const float* old_logp;          /* [dev][n]  log-probability under the policy that acted           */
+    const float* ref_logp;          /* [dev][n] or NULL: KL estimated from the frozen policy's log-probability of the action */
+    const float* weights;           /* [dev][n] or NULL: 1 / n each                                    */
+    const void* ref_logits;         /* [dev] or NULL: KL over the frozen policy's logits (same type)   */
+    int64_t ref_ld;
+    float clip_low, clip_high;      /* the ratio is clipped to [1 - clip_low, 1 + clip_high]           */
+    float kl_coef, entropy_coef;
+} qz_policy_terms;
+/* log-probability of the actions, [dev][n] float32; entropy and stats may be NULL; stats, [dev][2][n] float32: a row's largest
+ * legal logit and the logarithm of its sum of exponentials past it, what the backward pass needs.
+ * workspace: qz_policy_workspace bytes. */
+int64_t qz_policy_workspace(int64_t n, int n_actions);
+int qz_action_logp(const qz_policy_rows* rows, float* logp /*[dev]*/, float* entropy /*[dev] or NULL*/, float* stats /*[dev] or NULL*/,
+                   void* workspace /*[dev]*/, int64_t workspace_bytes, void* stream);
+/* grad (type of the logits, ld_grad elements between rows) <- dlogp[i] d logp_i + dentropy[i] d entropy_i; dlogp or dentropy may
+ * be NULL; entropy is the forward pass's (NULL only where dentropy is). */
+int qz_action_logp_backward(const qz_policy_rows* rows, const float* stats /*[dev]*/, const float* entropy /*[dev] or NULL*/,
+                            const float* dlogp /*[dev] or NULL*/, const float* dentropy /*[dev] or NULL*/, void* grad /*[dev]*/, int64_t ld_grad,
+                            void* stream);
+/* loss <- sum_i w_i [ -min(r A, clip(r) A) + kl_coef KL - entropy_coef H ], r = exp(logp - old_logp); per row logp, kl, entropy;
+ * grad <- d loss / d logits (NULL: loss only). */
+int qz_policy_loss(const qz_policy_rows* rows, const qz_policy_terms* terms, float* loss /*[dev][1]*/, float* logp /*[dev][n]*/,
+                   float* kl /*[dev][n]*/, float* entropy /*[dev][n]*/, void* grad /*[dev] or NULL*/, int64_t ld_grad, void* workspace /*[dev]*/,
+                   int64_t workspace_bytes, void* stream);
+/* grad <- *upstream x d loss / d logits, computed afresh (a rounded 16-bit gradient is not multiplied again: under a loss scale
+ * its small entries would be lost).  only_if_scaled != 0: leaves grad alone where *upstream is 1 (it already holds the answer). */
+int qz_policy_loss_backward(const qz_policy_rows* rows, const qz_policy_terms* terms, const float* upstream /*[dev][1]*/, int only_if_scaled,
+                            void* grad /*[dev]*/, int64_t ld_grad, void* workspace /*[dev]*/, int64_t workspace_bytes, void* stream);
+
+/* One matrix of a list (the list itself is host memory, read during the call). */
+typedef struct {
+    int64_t rows, cols;             /* 1 .. 1048576 each, 2^32 elements at most (a matrix with a zero side is skipped) */
+    const void* update;             /* [dev] the update to orthogonalise / the gradient                */
+    int64_t ld;                     /* elements between its rows                                       */
+    void* out;                      /* [dev] qz_orthogonalize: the result, same type                   */
+    int64_t out_ld;
+    float* momentum;                /* [dev] qz_muon_step: float32 [rows][cols], updated               */
+    float* param;                   /* [dev] qz_muon_step: float32 [rows][cols], updated               */
+    float scale;                    /* qz_muon_step: factor of the learning rate for this matrix       */
+} qz_matrix;
+typedef struct {
+    float lr, momentum, weight_decay;
+    int32_t nesterov;
+    const float* lr_dev;            /* [dev][1] or NULL: the learning rate in device memory (captured graphs follow it) */
+} qz_muon_opts;
+/* out <- the Newton-Schulz iterate of update / max(|update|_F, 1e-7) after `steps` (1 .. 16) quintic steps (3.4445, -4.7750,
+ * 2.0315): the singular vectors stay, the singular values move towards 1. */
+int64_t qz_orthogonalize_workspace(const qz_matrix* list /*[host]*/, int count);
+int qz_orthogonalize(const qz_matrix* list /*[host]*/, int count, int dtype, int steps, void* workspace /*[dev]*/, int64_t workspace_bytes,
+                     void* stream);
+/* momentum <- mu momentum + (1 - mu) G;  U = nesterov ? (1 - mu) G + mu momentum : momentum;
+ * param <- param (1 - lr weight_decay) - lr scale orthogonalize(U).  dtype: of the gradients. */
+int qz_muon_step(const qz_matrix* list /*[host]*/, int count, int dtype, int steps, const qz_muon_opts* opts, void* workspace /*[dev]*/,
+                 int64_t workspace_bytes, void* stream);
 
 /* self-test hook for the GPU tests: out[i] <- device sqrt((double)i), i < n.  The PUCT term
  * uses np.sqrt(parent visits) in float64 (mcts.py:69); the test checks the device result is
