@@ -1202,12 +1202,13 @@ static int run_matrices(const qz_matrix* list, int count, const OrthoStep& o, vo
 }
 int64_t qz_orthogonalize_workspace(const qz_matrix* list, int count) {
     if (count <= 0 || !list) return 0;
-    int64_t n = 0;
-    for (int i = 0; i < count; i++) {
-        const OrthoMatrix q = {list[i].rows, list[i].cols, nullptr, 0, nullptr, 0, nullptr, nullptr, 0.f};
-        n += qzl::ortho_workspace_bytes(&q, 1, OrthoStep{});
+    try {
+        std::vector<OrthoMatrix> q;
+        for (int i = 0; i < count; i++) q.push_back(OrthoMatrix{list[i].rows, list[i].cols, nullptr, 0, nullptr, 0, nullptr, nullptr, 0.f});
+        return qzl::ortho_workspace_bytes(q.data(), count, OrthoStep{});
+    } catch (const std::bad_alloc&) {
+        return fail(QZ_E_OOM, "out of host memory");
     }
-    return n;
 }
 int qz_orthogonalize(const qz_matrix* list, int count, int dtype, int steps, void* workspace, int64_t workspace_bytes, void* stream) {
     return run_matrices(list, count, OrthoStep{dtype, steps, 0, 0, 0.f, 0.f, 0.f, nullptr}, workspace, workspace_bytes, stream);
