@@ -27,7 +27,8 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
-constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f, NORM_FLOOR = 1e-7f;
+constexpr double NS_A_64 = 3.4445, NS_B_64 = -4.7750, NS_C_64 = 2.0315;
+constexpr float NS_A = (float)NS_A_64, NS_B = (float)NS_B_64, NS_C = (float)NS_C_64, NORM_FLOOR = 1e-7f;
 constexpr float SCALE = 4096.f, INV_SCALE = 1.f / 4096.f, INV_SCALE2 = 1.f / (4096.f * 4096.f);
 constexpr int MAX_MATS = 20;      // matrices per launch: their descriptors travel as kernel arguments (captured graphs keep them)
 constexpr int MAX_PARTS = 1024;    // partial sums of |U|^2 per matrix
@@ -465,18 +466,464 @@ __global__ __launch_bounds__(256) void k_ns_join(Mats M, Part part) {
     store_symmetric<KIND>(m, ti != tj, row, col, v);
 }
 
+// ================================================================ shorter side up to 128: one launch per step
+// A workgroup of eight waves owns a strip of 128 entries of the longer side through all steps, with the whole shorter side (S = 64 or
+// 128, zero padded).  Strips share nothing but A: every launch ends with each strip's part of the next A = X X^T (float32), and
+// begins with every workgroup summing the parts (in order) and forming B = b A + c A A for itself -- a 64^3 product done nine times
+// over costs less than the launches it replaces.  Then X' = a X + B X on its strip, from registers, and X' X'^T through LDS.
+// Bound by latencies one after the other (descriptor, parts from memory, LDS round trips), not by arithmetic.
+constexpr int STRIP = 128, STRIP_THREADS = 512;
+constexpr int STRIP_SUM = 65536;  // most floats of parts that a workgroup sums: 16 strips of 64 x 64, 4 of 128 x 128 (256 KB, ~2 us)
+constexpr int TINY = 16, TINY_LONG = 8192;
+
+struct StripShared {
+    union {
+        half8 a[2][128 * 128 / 8];     // A: [hi | lo][row, chunk of 8]
+        half8 xs[2][128 * STRIP / 8];  // then X': [hi | lo][row of the shorter side, chunk of 8 of the strip]
+        float out[128 * STRIP];        // or the result, [row of the shorter side][entry of the strip ^ row & 31]
+        double sum[STRIP_THREADS];
+        struct {
+            double red[STRIP_THREADS / 64][TINY * TINY], A[TINY][TINY + 1], B[TINY][TINY + 1], P[TINY][TINY + 1], Q[TINY][TINY + 1];
+        } tiny;
+    };
+    half8 b[2][128 * 128 / 8];         // B
+};
+template <int S>
+__device__ __forceinline__ int ab_at(int row, int chunk) {  // sixteen consecutive rows fall on sixteen bank groups
+    return row * (S / 8) + (chunk ^ (S == 64 ? (row >> 1) & 7 : row & 15));
+}
+__device__ __forceinline__ int xs_at(int row, int chunk) { return row * (STRIP / 8) + (chunk ^ (row & 15)); }
+// P Q^T with hi / lo operands: one accumulator per product, so that a wave is not bound by the latency of adding to the same
+// registers again
+struct Acc3 {
+    floatx16 a, b, c;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < 16; e++) a[e] = b[e] = c[e] = 0.f;
+    }
+    __device__ __forceinline__ void add(const half8& ph, const half8& pl, const half8& qh, const half8& ql) {
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, a, 0, 0, 0);
+        b = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, b, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ float get(int e) const { return (a[e] + b[e]) + c[e]; }
+};
+// lanes r | r + 32 hold chunks c | c + 1 of eight values each -> lane r: the lower halves of both, lane r + 32: the upper halves
+__device__ __forceinline__ void halves(const half8& v, half4& even, half4& odd) {
+    typedef uint32_t uint4_ __attribute__((ext_vector_type(4)));
+    typedef uint32_t uint2_ __attribute__((ext_vector_type(2)));
+    const uint4_ w = __builtin_bit_cast(uint4_, v);
+    const uint2_ a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    even = __builtin_bit_cast(half4, (uint2_){a[0], b[0]});
+    odd = __builtin_bit_cast(half4, (uint2_){a[1], b[1]});
+}
+// The parts of A: its lower tiles of 32 x 32 only (3 of 4, 10 of 16: a CU reads what other workgroups wrote at some 40 GB/s, and this is
+// most of what it reads), each [column][row].
+template <int S>
+constexpr int part_tiles() {
+    return S == 64 ? 3 : 10;
+}
+template <int S>
+constexpr int part_floats() {
+    return part_tiles<S>() * 1024;
+}
+__device__ __forceinline__ void part_tile(int t, int& ti, int& tj) {
+    ti = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0;
+    tj = t - ti * (ti + 1) / 2;
+}
+// this strip's part of X X^T, scaled by SCALE^2; a tile per wave, then two more
+template <int S>
+__device__ __forceinline__ void strip_gram(const StripShared& sm, float* __restrict__ part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, h = lane >> 5;
+#pragma unroll 1
+    for (int t = wave; t < part_tiles<S>(); t += STRIP_THREADS / 64) {
+        int ti, tj;
+        part_tile(t, ti, tj);
+        Acc3 acc;
+        acc.clear();
+#pragma unroll
+        for (int kk = 0; kk < STRIP / 16; kk++) {
+            const int p = xs_at(32 * ti + r32, 2 * kk + h), q = xs_at(32 * tj + r32, 2 * kk + h);
+            acc.add(sm.xs[0][p], sm.xs[1][p], sm.xs[0][q], sm.xs[1][q]);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<float4*>(part + t * 1024 + r32 * 32 + 8 * g + 4 * h) = make_float4(acc.get(4 * g), acc.get(4 * g + 1), acc.get(4 * g + 2), acc.get(4 * g + 3));
+    }
+}
+// four entries of the shorter side (s0 ..) of one entry l of the longer side: to X^T in memory and to X in LDS
+template <int S>
+__device__ __forceinline__ void strip_keep(StripShared& sm, _Float16* xt, int64_t plane, int l0, int l, int s0, const float (&v)[4]) {
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        _Float16 a, b;
+        split(v[e], a, b);
+        hi[e] = a;
+        lo[e] = b;
+        const int at = xs_at(s0 + e, l >> 3) * 8 + (l & 7);
+        reinterpret_cast<_Float16*>(sm.xs[0])[at] = a;
+        reinterpret_cast<_Float16*>(sm.xs[1])[at] = b;
+    }
+    *reinterpret_cast<half4*>(xt + (int64_t)(l0 + l) * S + s0) = hi;
+    *reinterpret_cast<half4*>(xt + plane + (int64_t)(l0 + l) * S + s0) = lo;
+}
+
+template <int S>
+__device__ __forceinline__ void strip_first(const Mats& M, const Mat& m, int strip, StripShared& sm) {
+    double s = 0.0;
+    for (int k = threadIdx.x; k < m.nparts; k += STRIP_THREADS) s += m.parts[k];
+    sm.sum[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = STRIP_THREADS / 2; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) sm.sum[threadIdx.x] += sm.sum[threadIdx.x + o];
+        __syncthreads();
+    }
+    const double norm = sqrt(sm.sum[0]);
+    const float inv = (float)(1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm));
+    __syncthreads();
+    const bool tall = m.rows > m.cols;
+    const void* src = M.o.muon ? (const void*)m.xt1 : m.update;
+    const int64_t ld = M.o.muon ? m.cols : m.ld, plane = (int64_t)S * m.lp;
+    const int dtype = M.o.muon ? 0 : M.o.dtype, smax = tall ? m.cols : m.rows, lmax = tall ? m.rows : m.cols;
+    const int l0 = strip * STRIP, l = threadIdx.x & 127;
+#pragma unroll 1
+    for (int s0 = (threadIdx.x >> 7) * 4; s0 < S; s0 += 64) {  // sixteen loads in flight per thread
+        float v[4][4];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int si = s0 + 16 * q + e;
+                v[q][e] = 0.f;
+                if (si < smax && l0 + l < lmax) v[q][e] = load_elem(src, tall ? (int64_t)(l0 + l) * ld + si : (int64_t)si * ld + l0 + l, dtype) * inv;
+            }
+#pragma unroll
+        for (int q = 0; q < 4; q++) strip_keep<S>(sm, m.xt0, plane, l0, l, s0 + 16 * q, v[q]);
+    }
+    __syncthreads();
+    strip_gram<S>(sm, reinterpret_cast<float*>(m.a) + (int64_t)strip * part_floats<S>());
+}
+
+template <int S>
+__device__ __forceinline__ void strip_step(const Mats& M, const Mat& m, int strip, int odd, int last, StripShared& sm) {
+    constexpr int NK = S / 16, NJ = (part_floats<S>() / 4 + STRIP_THREADS - 1) / STRIP_THREADS, NP = S == 64 ? 8 : 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, h = lane >> 5;
+    const int l0 = strip * STRIP, lw = (wave & 3) * 32 + r32, strips = m.lp / STRIP;
+    const int64_t plane = (int64_t)S * m.lp;
+    const _Float16* xt = (odd ? m.xt1 : m.xt0) + (int64_t)(l0 + lw) * S;
+    half8 xh[NK], xl[NK];
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        xh[k] = *reinterpret_cast<const half8*>(xt + 16 * k + 8 * h);
+        xl[k] = *reinterpret_cast<const half8*>(xt + plane + 16 * k + 8 * h);
+    }
+    {  // A, from the strips' parts: 16 (20) 16-byte loads in flight per thread
+        const float4* part = reinterpret_cast<const float4*>(odd ? m.b : m.a);
+        float sum[NJ][4] = {};
+#pragma unroll 1
+        for (int p = 0; p < strips; p += NP) {
+            float4 u[NP][NJ];
+#pragma unroll
+            for (int q = 0; q < NP; q++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const int e0 = threadIdx.x + STRIP_THREADS * j;
+                    u[q][j] = part[(int64_t)(p + q < strips ? p + q : p) * (part_floats<S>() / 4) + (e0 < part_floats<S>() / 4 ? e0 : 0)];
+                }
+#pragma unroll
+            for (int q = 0; q < NP; q++) {
+                if (p + q < strips) {
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        sum[j][0] += u[q][j].x;
+                        sum[j][1] += u[q][j].y;
+                        sum[j][2] += u[q][j].z;
+                        sum[j][3] += u[q][j].w;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int e0 = threadIdx.x + STRIP_THREADS * j;
+            if (e0 >= part_floats<S>() / 4) continue;
+            int ti, tj;
+            part_tile(e0 >> 8, ti, tj);
+            const int row = 32 * ti + (e0 & 7) * 4, col = 32 * tj + ((e0 & 255) >> 3);  // four rows of a column
+            half4 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                _Float16 a, b;
+                split(sum[j][e] * INV_SCALE2, a, b);
+                hi[e] = a;
+                lo[e] = b;
+                if (ti != tj) {
+                    const int at = ab_at<S>(row + e, col >> 3) * 8 + (col & 7);
+                    reinterpret_cast<_Float16*>(sm.a[0])[at] = a;
+                    reinterpret_cast<_Float16*>(sm.a[1])[at] = b;
+                }
+            }
+            const int at = ab_at<S>(col, row >> 3) * 2 + ((row >> 2) & 1);
+            reinterpret_cast<half4*>(sm.a[0])[at] = hi;
+            reinterpret_cast<half4*>(sm.a[1])[at] = lo;
+        }
+    }
+    __syncthreads();
+    // B = b A + c A A, all tiles (S = 64: one for each of four waves; S = 128: two per wave)
+    if (S == 128 || wave < 4) {
+        const int ti = wave >> 1;
+#pragma unroll 1
+        for (int y = 0; y < (S == 64 ? 1 : 2); y++) {
+            const int tj = S == 64 ? wave & 1 : 2 * (wave & 1) + y;
+            Acc3 acc;
+            acc.clear();
+#pragma unroll
+            for (int k = 0; k < NK; k++) {
+                const int p = ab_at<S>(32 * ti + r32, 2 * k + h), q = ab_at<S>(32 * tj + r32, 2 * k + h);
+                acc.add(sm.a[0][p], sm.a[1][p], sm.a[0][q], sm.a[1][q]);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; g++) {  // rows 32 ti + 8 g + 4 h .. of column 32 tj + r32; A is symmetric
+                const int at = ab_at<S>(32 * tj + r32, 4 * ti + g) * 2 + h;
+                const half4 ah = reinterpret_cast<const half4*>(sm.a[0])[at], al = reinterpret_cast<const half4*>(sm.a[1])[at];
+                half4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    _Float16 a, b;
+                    split(NS_B * (((float)ah[e] + (float)al[e]) * INV_SCALE) + NS_C * (acc.get(4 * g + e) * INV_SCALE2), a, b);
+                    hi[e] = a;
+                    lo[e] = b;
+                }
+                reinterpret_cast<half4*>(sm.b[0])[at] = hi;
+                reinterpret_cast<half4*>(sm.b[1])[at] = lo;
+            }
+        }
+    }
+    __syncthreads();
+    // X' = a X + B X: rows = the shorter side (waves 4 .. 7 its upper half), columns = 32 entries of the longer one
+#pragma unroll
+    for (int t = 0; t < S / 64; t++) {
+        const int y = t + (wave >> 2) * (S / 64);
+        // This lane's entries of the old X: of each chunk of eight, the half that its results lie in.  Lanes r and r + 32 hold chunk
+        // 2 k and 2 k + 1; swapping the one's upper with the other's lower half gives both what they need.
+        half4 oh[4], ol[4];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            half8 vh = xh[2 * t + k], vl = xl[2 * t + k];
+            const half8 uh = xh[2 * (t + S / 64) + k], ul = xl[2 * (t + S / 64) + k];
+            if (wave >> 2) {
+                vh = uh;
+                vl = ul;
+            }
+            halves(vh, oh[2 * k], oh[2 * k + 1]);
+            halves(vl, ol[2 * k], ol[2 * k + 1]);
+        }
+        Acc3 c;
+        c.clear();
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const int p = ab_at<S>(32 * y + r32, 2 * k + h);
+            c.add(sm.b[0][p], sm.b[1][p], xh[k], xl[k]);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int s0 = 32 * y + 8 * g + 4 * h;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = NS_A * (((float)oh[g][e] + (float)ol[g][e]) * INV_SCALE) + c.get(4 * g + e) * INV_SCALE2;
+            if (!last) {
+                strip_keep<S>(sm, odd ? m.xt0 : m.xt1, plane, l0, lw, s0, v);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) sm.out[(s0 + e) * STRIP + (lw ^ ((s0 + e) & 31))] = v[e];
+            }
+        }
+    }
+    __syncthreads();
+    if (!last) {
+        strip_gram<S>(sm, reinterpret_cast<float*>(odd ? m.a : m.b) + (int64_t)strip * part_floats<S>());
+        return;
+    }
+    const bool tall = m.rows > m.cols;
+    const int smax = tall ? m.cols : m.rows, lmax = tall ? m.rows : m.cols;
+    const float lr = M.o.muon ? (M.o.lr_dev ? *M.o.lr_dev : M.o.lr) : 0.f;
+#pragma unroll 1
+    for (int e0 = threadIdx.x; e0 < S * STRIP; e0 += 8 * STRIP_THREADS) {  // along the rows of the result, eight weights in flight
+        float w[8], v[8];
+        int64_t at[8];
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            const int e = e0 + q * STRIP_THREADS, si = tall ? e % S : e / STRIP, l = tall ? e / S : e % STRIP;
+            const int64_t r = tall ? l0 + l : si, c = tall ? si : l0 + l;
+            const bool in = si < smax && l0 + l < lmax;
+            v[q] = sm.out[si * STRIP + (l ^ (si & 31))];
+            at[q] = in ? r * (M.o.muon ? m.cols : m.out_ld) + c : -1;
+            w[q] = M.o.muon && in ? m.param[at[q]] : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            if (at[q] < 0) continue;
+            if (M.o.muon) m.param[at[q]] = w[q] * (1.f - lr * M.o.weight_decay) - lr * m.scale * v[q];
+            else store_elem(m.out, at[q], M.o.dtype, v[q]);
+        }
+    }
+}
+
+// ---- shorter side up to 16: everything in one workgroup, float64
+// With X_k = P_k U / |U| only the s x s matrices move: A = U U^T / |U|^2 once, then A <- Q A Q, P <- Q P with Q = a + b A + c A A, and
+// X = P U / |U| at the end: 2 s^2 l products instead of 15 s^2 l.  In float32 this loses the small singular values (A holds their
+// squares, and its rounding error is carried by a^2 a step); in float64 it is more exact than the products on X.  The sum over l
+// runs on the float64 matrix instruction (16 x 16 x 4, both operands the same register; row (lane >> 4) + 4 e of column lane & 15),
+// bound by the latency of reading U.
+__device__ __forceinline__ void tiny_all(const Mats& M, const Mat& m, StripShared& shared) {
+    typedef double double4_ __attribute__((ext_vector_type(4)));
+    auto& sm = shared.tiny;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const bool tall = m.rows > m.cols;
+    const int s = tall ? m.cols : m.rows, l = tall ? m.rows : m.cols, size = s * l;
+    float* u = reinterpret_cast<float*>(m.xt1);  // [s][l]
+#pragma unroll 1
+    for (int e0 = tid; e0 < size; e0 += 4 * STRIP_THREADS) {  // four elements' loads in flight per thread
+        float v[4], old[4];
+        int at[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int e = e0 + STRIP_THREADS * q < size ? e0 + STRIP_THREADS * q : e0, r = e / m.cols, c = e - r * m.cols;
+            v[q] = load_elem(m.update, r * m.ld + c, M.o.dtype);
+            old[q] = M.o.muon ? m.momentum[e] : 0.f;
+            at[q] = tall ? c * l + r : e;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (e0 + STRIP_THREADS * q >= size) continue;
+            if (M.o.muon) {
+                const float mom = old[q] + (v[q] - old[q]) * (1.f - M.o.momentum);
+                m.momentum[e0 + STRIP_THREADS * q] = mom;
+                v[q] = M.o.nesterov ? v[q] + (mom - v[q]) * M.o.momentum : mom;
+            }
+            u[at[q]] = v[q];
+        }
+    }
+    __syncthreads();
+    const int row = lane & 15, kq = lane >> 4;
+    double4_ acc = {0.0, 0.0, 0.0, 0.0};
+    for (int k0 = __builtin_amdgcn_readfirstlane(wave) * 32; k0 < l; k0 += STRIP_THREADS / 2) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = row < s && k0 + 4 * k + kq < l ? u[row * l + k0 + 4 * k + kq] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v[k], (double)v[k], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) sm.red[wave][((lane >> 4) + 4 * e) * TINY + row] = acc[e];
+    __syncthreads();
+    const int i = (tid >> 4) & 15, j = tid & 15;  // (both halves of the workgroup compute, the first writes)
+    const bool mine = tid < TINY * TINY;
+    double g = 0.0;
+#pragma unroll
+    for (int w = 0; w < STRIP_THREADS / 64; w++) g += sm.red[w][i * TINY + j];
+    if (mine) sm.A[i][j] = g;
+    __syncthreads();
+    double norm2 = 0.0;
+    for (int k = 0; k < s; k++) norm2 += sm.A[k][k];
+    const double norm = sqrt(norm2), inv = 1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm);
+    __syncthreads();
+    if (mine) {
+        sm.A[i][j] = g * inv * inv;
+        sm.P[i][j] = i == j ? inv : 0.0;
+    }
+    __syncthreads();
+    auto product = [&](const double (&x)[TINY][TINY + 1], const double (&y)[TINY][TINY + 1]) {
+        double t = 0.0;
+        for (int k = 0; k < s; k++) t += x[i][k] * y[k][j];
+        return t;
+    };
+    for (int step = 0; step < M.o.steps; step++) {
+        const double q = (i == j ? NS_A_64 : 0.0) + NS_B_64 * sm.A[i][j] + NS_C_64 * product(sm.A, sm.A);
+        if (mine) sm.Q[i][j] = q;
+        __syncthreads();
+        const double p = product(sm.Q, sm.P), t = product(sm.Q, sm.A);
+        if (mine) sm.B[i][j] = t;
+        __syncthreads();
+        const double a = product(sm.B, sm.Q);
+        if (mine) {
+            sm.P[i][j] = p;
+            sm.A[i][j] = a;
+        }
+        __syncthreads();
+    }
+    const float lr = M.o.muon ? (M.o.lr_dev ? *M.o.lr_dev : M.o.lr) : 0.f;
+#pragma unroll 1
+    for (int e0 = tid; e0 < size; e0 += 4 * STRIP_THREADS) {
+        double t[4] = {0.0, 0.0, 0.0, 0.0};
+        int ss[4], ll[4];
+        float w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int e = e0 + STRIP_THREADS * q < size ? e0 + STRIP_THREADS * q : e0, r = e / m.cols, c = e - r * m.cols;
+            ss[q] = tall ? c : r;
+            ll[q] = tall ? r : c;
+            w[q] = M.o.muon ? m.param[e] : 0.f;
+        }
+        for (int k = 0; k < s; k++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) t[q] += sm.P[ss[q]][k] * (double)u[k * l + ll[q]];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int e = e0 + STRIP_THREADS * q;
+            if (e >= size) continue;
+            if (M.o.muon) m.param[e] = w[q] * (1.f - lr * M.o.weight_decay) - lr * m.scale * (float)t[q];
+            else store_elem(m.out, (int64_t)(e / m.cols) * m.out_ld + e % m.cols, M.o.dtype, (float)t[q]);
+        }
+    }
+}
+
+// first: X_0 and the parts of A, and the tiny matrices from beginning to end; else one step of the strips
+// Workgroup b runs on XCD b mod 8.  All strips of a matrix are given to one XCD, so that the parts one workgroup wrote are in the L2
+// that the others read them from: place (b mod 8) cap + b / 8, where each XCD has cap places; the tiny matrices come behind them.
+__global__ __launch_bounds__(STRIP_THREADS) void k_ns_strip(Mats M, int first, int odd, int last, int cap) {
+    __shared__ StripShared sm;
+    const int b = blockIdx.x, place = b < 8 * cap ? (b & 7) * cap + (b >> 3) : b;
+    if (place < M.start[0]) return;
+    const int i = find_mat(M, place);
+    const Mat& m = M.m[i];
+    const int strip = place - M.start[i];
+    if (strip >= (m.sp == TINY ? 1 : m.lp / STRIP)) return;  // an empty place
+    if (m.sp == TINY) {
+        tiny_all(M, m, sm);
+    } else if (m.sp == 64) {
+        if (first) strip_first<64>(M, m, strip, sm);
+        else strip_step<64>(M, m, strip, odd, last, sm);
+    } else {
+        if (first) strip_first<128>(M, m, strip, sm);
+        else strip_step<128>(M, m, strip, odd, last, sm);
+    }
+}
+
 // ================================================================ host side
 int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
+// How a matrix is worked on, by its sides alone.
+enum { PATH_TINY = 0, PATH_STRIP = 1, PATH_TILES = 2 };
+int path_of(int64_t rows, int64_t cols) {
+    const int64_t s = rows < cols ? rows : cols, l = rows < cols ? cols : rows;
+    if (s <= TINY && l <= TINY_LONG) return PATH_TINY;
+    const int64_t sp = s <= 64 ? 64 : 128;
+    return s <= 128 && (l + STRIP - 1) / STRIP * sp * sp <= STRIP_SUM ? PATH_STRIP : PATH_TILES;
+}
 // Matrices whose shorter side is 512 or more are padded so that tiles of 128 may be used.
 int pad_of(int64_t rows, int64_t cols) { return (rows < cols ? rows : cols) >= 512 ? 128 : 64; }
 bool one_product(const OrthoMatrix& q, const OrthoStep& o) { return !o.muon && o.dtype == 1 && (q.rows < q.cols ? q.rows : q.cols) >= 256; }
 
 int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
     const int64_t s = q.rows < q.cols ? q.rows : q.cols, l = q.rows < q.cols ? q.cols : q.rows;
-    const int T = pad_of(q.rows, q.cols);
-    const int64_t sp = align_up(s, T), lp = align_up(l, T);
-    const int64_t xb = align_up(sp * lp * 4, 256), ab = align_up(sp * sp * 4, 256), pb = MAX_PARTS * 8;
+    const int path = path_of(q.rows, q.cols), T = path == PATH_TINY ? TINY : path == PATH_STRIP ? (s <= 64 ? 64 : 128) : pad_of(q.rows, q.cols);
+    const int64_t sp = align_up(s, T), lp = align_up(l, path == PATH_STRIP ? STRIP : T);
+    // planes of X, and of A and B: (strips) X^T twice, U in the second's place, and two sets of parts of A; (tiny) U alone
+    const int64_t xb = path == PATH_TINY ? align_up(s * l * 4, 256) : align_up(sp * lp * 4, 256);
+    const int64_t ab = path == PATH_TINY ? 0 : align_up(sp * sp * 4 * (path == PATH_STRIP ? lp / STRIP : 1), 256), pb = MAX_PARTS * 8;
+    const int64_t xs = path == PATH_TINY ? 1 : path == PATH_STRIP ? 2 : 3;
     if (m) {
         const int64_t parts = (q.rows * q.cols + 4095) / 4096;
         m->update = q.update;
@@ -484,11 +931,12 @@ int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
         m->momentum = q.momentum;
         m->param = q.param;
         m->x = reinterpret_cast<_Float16*>(base);
-        m->xt0 = reinterpret_cast<_Float16*>(base + xb);
-        m->xt1 = reinterpret_cast<_Float16*>(base + 2 * xb);
-        m->a = reinterpret_cast<_Float16*>(base + 3 * xb);
-        m->b = reinterpret_cast<_Float16*>(base + 3 * xb + ab);
-        m->parts = reinterpret_cast<double*>(base + 3 * xb + 2 * ab);
+        m->xt0 = reinterpret_cast<_Float16*>(base + (path == PATH_TILES ? xb : 0));
+        m->xt1 = reinterpret_cast<_Float16*>(base + (xs - 1) * xb);
+        m->a = reinterpret_cast<_Float16*>(base + xs * xb);
+        m->b = reinterpret_cast<_Float16*>(base + xs * xb + ab);
+        m->parts = reinterpret_cast<double*>(base + xs * xb + 2 * ab);
+        m->pbase = 0;
         m->ld = q.ld;
         m->out_ld = q.out_ld;
         m->scale = q.scale;
@@ -498,7 +946,7 @@ int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
         m->lp = (int32_t)lp;
         m->nparts = (int32_t)(parts < MAX_PARTS ? parts : MAX_PARTS);
     }
-    return 3 * xb + 2 * ab + pb;
+    return xs * xb + 2 * ab + pb;
 }
 
 // A symmetric product of fewer tiles than this is split along K, into about SPLIT_GOAL workgroups of at least SPLIT_MIN stages: alone
@@ -570,6 +1018,47 @@ hipError_t run_steps(Mats& M, bool may128, float* partial, hipStream_t s) {
     return hipGetLastError();
 }
 
+// strips and tiny matrices, the tiny ones (shortest: lp is theirs too) behind the strips
+hipError_t run_strips(Mats& M, hipStream_t s) {
+    const int all = M.count;
+    int strips = 0, wgs = 0;
+    while (strips < all && M.m[strips].sp != TINY) strips++;
+    M.count = strips;
+    for (int i = 0; i < strips; i++) {
+        M.start[i] = wgs;
+        wgs += M.m[i].nparts;
+    }
+    if (strips) hipLaunchKernelGGL(k_ns_prepare, dim3(wgs), dim3(256), 0, s, M);
+    // the longest matrix first, to the XCD with the fewest strips; then in order of place
+    int load[8] = {}, xcd[MAX_MATS], cap = 0, n = 0;
+    for (int i = 0; i < strips; i++) {
+        int x = 0;
+        for (int k = 1; k < 8; k++)
+            if (load[k] < load[x]) x = k;
+        xcd[i] = x;
+        load[x] += M.m[i].lp / STRIP;
+        cap = load[x] > cap ? load[x] : cap;
+    }
+    Mats R = M;
+    for (int x = 0; x < 8; x++) {
+        int at = x * cap;
+        for (int i = 0; i < strips; i++)
+            if (xcd[i] == x) {
+                R.m[n] = M.m[i];
+                R.start[n++] = at;
+                at += M.m[i].lp / STRIP;
+            }
+    }
+    for (int i = strips; i < all; i++) R.start[i] = 8 * cap + (i - strips);
+    R.count = all;
+    hipLaunchKernelGGL(k_ns_strip, dim3(8 * cap + (all - strips)), dim3(STRIP_THREADS), 0, s, R, 1, 0, 0, cap);
+    R.count = strips;
+    for (int step = 0; step < M.o.steps && strips; step++)
+        hipLaunchKernelGGL(k_ns_strip, dim3(8 * cap), dim3(STRIP_THREADS), 0, s, R, 0, step & 1, step + 1 == M.o.steps, cap);
+    M.count = all;
+    return hipGetLastError();
+}
+
 hipError_t run_group(Mats& M, int pad, bool one, float* partial, hipStream_t s) {
     int wgs = 0;
     for (int i = 0; i < M.count; i++) {
@@ -593,6 +1082,7 @@ int64_t partial_bytes(const OrthoMatrix* q, int count) {
     for (int i = 0; i < count; i++) {
         if (q[i].rows <= 0 || q[i].cols <= 0) continue;
         const int64_t s = q[i].rows < q[i].cols ? q[i].rows : q[i].cols, l = q[i].rows < q[i].cols ? q[i].cols : q[i].rows;
+        if (path_of(q[i].rows, q[i].cols) != PATH_TILES) continue;
         const int64_t pad = pad_of(q[i].rows, q[i].cols);
         if (pad == 128) most = (int64_t)(SPLIT_GOAL + SLOTS) * 128 * 128 * 4;
         const int64_t t = align_up(s, pad) / 64, nk = align_up(l, pad) / BK;
@@ -614,35 +1104,43 @@ int64_t ortho_workspace_bytes(const OrthoMatrix* q, int count, const OrthoStep&)
 }
 
 hipError_t orthogonalize(const OrthoMatrix* q, int count, const OrthoStep& o, void* ws, hipStream_t s) {
-    // matrices of one padding and precision share their launches
-    for (int pad = 64; pad <= 128; pad += 64)
-        for (int one = 0; one < 2; one++) {
-            Mats M;
-            M.o = o;
+    // groups that share their launches: strips and tiny ones, and tiles of either padding and precision
+    float* partial = static_cast<float*>(ws);
+    for (int group = 0; group < 5; group++) {
+        const bool tiles = group > 0, one = tiles && (group - 1) & 1;
+        const int pad = group <= 2 ? 64 : 128;
+        Mats M;
+        M.o = o;
+        M.count = 0;
+        char* base = static_cast<char*>(ws) + partial_bytes(q, count);
+        auto run = [&]() -> hipError_t {
+            const hipError_t e = tiles ? run_group(M, pad, one, partial, s) : run_strips(M, s);
             M.count = 0;
-            float* partial = static_cast<float*>(ws);
-            char* base = static_cast<char*>(ws) + partial_bytes(q, count);
-            for (int i = 0; i < count; i++) {
-                if (q[i].rows <= 0 || q[i].cols <= 0) continue;
-                if (pad_of(q[i].rows, q[i].cols) == pad && one_product(q[i], o) == (one != 0)) {
-                    Mat m;
-                    layout(q[i], base, &m);
-                    int at = M.count++;  // longest first: their workgroups run longest
-                    for (; at > 0 && M.m[at - 1].lp < m.lp; at--) M.m[at] = M.m[at - 1];
-                    M.m[at] = m;
-                    if (M.count == MAX_MATS) {
-                        const hipError_t e = run_group(M, pad, one != 0, partial, s);
-                        if (e != hipSuccess) return e;
-                        M.count = 0;
-                    }
+            return e;
+        };
+        for (int i = 0; i < count; i++) {
+            if (q[i].rows <= 0 || q[i].cols <= 0) continue;
+            const bool in_tiles = path_of(q[i].rows, q[i].cols) == PATH_TILES;
+            if (in_tiles == tiles && (!tiles || (pad_of(q[i].rows, q[i].cols) == pad && one_product(q[i], o) == one))) {
+                Mat m;
+                layout(q[i], base, &m);
+                // longest first: their workgroups run longest; tiny ones at the end
+                const int64_t key = m.sp == TINY ? 0 : m.lp;
+                int at = M.count++;
+                for (; at > 0 && (M.m[at - 1].sp == TINY ? 0 : M.m[at - 1].lp) < key; at--) M.m[at] = M.m[at - 1];
+                M.m[at] = m;
+                if (M.count == MAX_MATS) {
+                    const hipError_t e = run();
+                    if (e != hipSuccess) return e;
                 }
-                base += layout(q[i], nullptr, nullptr);
             }
-            if (M.count) {
-                const hipError_t e = run_group(M, pad, one != 0, partial, s);
-                if (e != hipSuccess) return e;
-            }
+            base += layout(q[i], nullptr, nullptr);
         }
+        if (M.count) {
+            const hipError_t e = run();
+            if (e != hipSuccess) return e;
+        }
+    }
     return hipSuccess;
 }
 }  // namespace qzl
