@@ -50,7 +50,7 @@ def _rows_of(logits, name="logits"):
         raise TypeError("%s: %s is not one of float32, bfloat16, float16" % (name, logits.dtype))
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("%s: at least one action is needed, got the shape %s" % (name, tuple(logits.shape)))
-    return logits.reshape(-1, logits.shape[-1])
+    return logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
 
 
 def _unit_rows(t):
@@ -69,6 +69,8 @@ def _vector(t, lead, device, name):
         raise TypeError("%s must be floating point" % name)
     if tuple(t.shape) != tuple(lead):
         raise ValueError("%s has the shape %s, %s is needed" % (name, tuple(t.shape), tuple(lead)))
+    if t.dtype is torch.float32 and t.dim() == 1 and t.is_contiguous():
+        return t
     return t.to(torch.float32).reshape(-1).contiguous()
 
 
@@ -78,6 +80,8 @@ def _actions(t, lead, device):
         raise TypeError("actions must be integers")
     if tuple(t.shape) != tuple(lead):
         raise ValueError("actions have the shape %s, %s is needed" % (tuple(t.shape), tuple(lead)))
+    if t.dtype is torch.int64 and t.dim() == 1 and t.is_contiguous():
+        return t
     return t.to(torch.int64).reshape(-1).contiguous()
 
 
@@ -91,7 +95,9 @@ def _legal(t, lead, a, device):
         raise TypeError("legal: %s is neither packed 32-bit words nor bytes" % t.dtype)
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError("legal has the shape %s, its last dimension must be %d" % (tuple(t.shape), width))
-    return _unit_rows(t.expand(tuple(lead) + (width,)).reshape(-1, width)), kind
+    if t.dim() != 2 or len(lead) != 1 or t.shape[0] != lead[0]:
+        t = t.expand(tuple(lead) + (width,)).reshape(-1, width)
+    return _unit_rows(t), kind
 
 
 def _struct(z, actions, legal, kind):
@@ -101,11 +107,6 @@ def _struct(z, actions, legal, kind):
 
 def _ptr(t):
     return t.data_ptr() if t is not None else 0
-
-
-def _workspace(n, a, device):
-    size = _cabi.load().qz_policy_workspace(n, a)
-    return torch.empty(max(size, 1), dtype=torch.uint8, device=device), size
 
 
 class _Launch:
@@ -125,6 +126,17 @@ class _Launch:
             self.guard.__exit__(*exc)
 
 
+def _call(device, fn, *args):
+    """fn(*args, stream) of the library on the device's current stream (a raw handle: wrapping it in a Stream costs 3 us)."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with _Launch(device) as stream:
+            rc = fn(*args, stream)
+    if rc:
+        _cabi.check(rc)
+
+
 def _refuse_captured_leaf(logits):
     # the backward pass of a leaf runs on the stream that the leaf's gradient was first accumulated on: inside a capture that
     # may be a stream outside of it, which ends the process
@@ -138,17 +150,12 @@ class _ActionLogp(torch.autograd.Function):
     def forward(ctx, z, actions, legal, kind, want_entropy):
         n, a = z.shape
         z = _unit_rows(z)
-        logp = torch.empty(n, dtype=torch.float32, device=z.device)
         need = ctx.needs_input_grad[0]
-        entropy = torch.empty_like(logp) if want_entropy else None
-        stats = torch.empty((2, n), dtype=torch.float32, device=z.device) if need else None
-        ws, size = _workspace(n, a, z.device)
-        with _Launch(z.device) as stream:
-            _cabi.check(_cabi.load().qz_action_logp(C.byref(_struct(z, actions, legal, kind)), logp.data_ptr(), _ptr(entropy), _ptr(stats), ws.data_ptr(),
-                                                    size, stream))
-        ctx.kind = kind
-        ctx.save_for_backward(z, actions, legal, stats, entropy)
-        ctx.set_materialize_grads(False)
+        logp, entropy, stats = _logp(z, actions, legal, kind, want_entropy, need)
+        if need:
+            ctx.kind = kind
+            ctx.save_for_backward(z, actions, legal, stats, entropy)
+            ctx.set_materialize_grads(False)
         return (logp, entropy) if want_entropy else logp
 
     @staticmethod
@@ -160,10 +167,21 @@ class _ActionLogp(torch.autograd.Function):
         dlogp = dlogp.contiguous() if dlogp is not None else None
         dentropy = dentropy.contiguous() if dentropy is not None else None
         grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        with _Launch(z.device) as stream:
-            _cabi.check(_cabi.load().qz_action_logp_backward(C.byref(_struct(z, actions, legal, ctx.kind)), stats.data_ptr(), _ptr(entropy), _ptr(dlogp),
-                                                             _ptr(dentropy), grad.data_ptr(), grad.stride(0), stream))
+        _call(z.device, _cabi.load().qz_action_logp_backward, _struct(z, actions, legal, ctx.kind), stats.data_ptr(), _ptr(entropy), _ptr(dlogp),
+              _ptr(dentropy), grad.data_ptr(), z.shape[1])
         return grad, None, None, None, None
+
+
+def _logp(z, actions, legal, kind, want_entropy, want_stats):
+    n, a = z.shape
+    logp = torch.empty(n, dtype=torch.float32, device=z.device)
+    entropy = torch.empty_like(logp) if want_entropy else None
+    stats = torch.empty((2, n), dtype=torch.float32, device=z.device) if want_stats else None
+    L = _cabi.load()
+    size = L.qz_policy_workspace(n, a)
+    ws = torch.empty(size, dtype=torch.uint8, device=z.device) if size else None
+    _call(z.device, L.qz_action_logp, _struct(z, actions, legal, kind), logp.data_ptr(), _ptr(entropy), _ptr(stats), _ptr(ws), size)
+    return logp, entropy, stats
 
 
 def action_logp(logits, actions, legal=None, entropy=False):
@@ -174,10 +192,14 @@ def action_logp(logits, actions, legal=None, entropy=False):
     _refuse_captured_leaf(logits)
     acts = _actions(actions, lead, z.device)
     mask, kind = _legal(legal, lead, z.shape[1], z.device)
-    out = _ActionLogp.apply(z, acts, mask, kind, bool(entropy))
-    if entropy:
-        return out[0].reshape(lead), out[1].reshape(lead)
-    return out.reshape(lead)
+    if z.requires_grad and torch.is_grad_enabled():
+        out = _ActionLogp.apply(z, acts, mask, kind, bool(entropy))
+        logp, ent = out if entropy else (out, None)
+    else:
+        logp, ent, _ = _logp(_unit_rows(z), acts, mask, kind, bool(entropy), False)
+    if len(lead) != 1:
+        logp, ent = logp.reshape(lead), ent.reshape(lead) if entropy else None
+    return (logp, ent) if entropy else logp
 
 
 class _Terms(NamedTuple):
@@ -193,16 +215,21 @@ class _Terms(NamedTuple):
 
 
 def _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, want_grad):
+    """-> loss, logp, kl, entropy, gradient or None, and the call's two structs and its workspace (the backward pass's too)."""
     n, a = z.shape
-    row = torch.empty((3, n), dtype=torch.float32, device=z.device)
-    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    L = _cabi.load()
+    size = L.qz_policy_workspace(n, a)
+    head = (size + 15) & ~15
+    # one allocation: workspace | logp | kl | entropy | loss
+    buf = torch.empty(head + 12 * n + 4, dtype=torch.uint8, device=z.device)
+    logp, kl, entropy, loss = buf[head:].view(torch.float32).split([n, n, n, 1])
+    loss = loss.view(())
     grad = torch.empty((n, a), dtype=z.dtype, device=z.device) if want_grad else None
-    ws, size = _workspace(n, a, z.device)
-    t = terms.struct(advantages, old_logp, ref_logp, weights, ref)
-    with _Launch(z.device) as stream:
-        _cabi.check(_cabi.load().qz_policy_loss(C.byref(_struct(z, actions, legal, terms.kind)), C.byref(t), loss.data_ptr(), row[0].data_ptr(),
-                                                row[1].data_ptr(), row[2].data_ptr(), _ptr(grad), a, ws.data_ptr(), size, stream))
-    return loss, row[0], row[1], row[2], grad
+    rows, t = _struct(z, actions, legal, terms.kind), terms.struct(advantages, old_logp, ref_logp, weights, ref)
+    at = buf.data_ptr()
+    out = at + head
+    _call(z.device, L.qz_policy_loss, rows, t, out + 12 * n, out, out + 4 * n, out + 8 * n, _ptr(grad), a, at, size)
+    return loss, logp, kl, entropy, grad, (rows, t, buf, size)
 
 
 class _ClippedPolicyLoss(torch.autograd.Function):
@@ -212,27 +239,27 @@ class _ClippedPolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms):
         z = _unit_rows(z)
-        loss, logp, kl, entropy, grad = _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, ctx.needs_input_grad[0])
-        ctx.terms, ctx.grad = terms, grad
+        loss, logp, kl, entropy, ctx.grad, ctx.call = _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, True)
         ctx.save_for_backward(z, actions, legal, advantages, old_logp, ref_logp, weights, ref)
         ctx.mark_non_differentiable(logp, kl, entropy)
+        ctx.set_materialize_grads(False)
         return loss, logp, kl, entropy
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, *_):
-        z, actions, legal, advantages, old_logp, ref_logp, weights, ref = ctx.saved_tensors
+        z = ctx.saved_tensors[0]  # (checks that none of them was changed in place; the structs hold their addresses)
+        if upstream is None:
+            return (None,) * 9
+        rows, t, ws, size = ctx.call
         grad, ctx.grad = ctx.grad, None
-        fresh = grad is None
-        if fresh:
+        kept = grad is not None
+        if not kept:  # a second backward pass: computed again, with a workspace of its own
             grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        ws, size = _workspace(z.shape[0], z.shape[1], z.device)
-        t = ctx.terms.struct(advantages, old_logp, ref_logp, weights, ref)
+            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=z.device)
         upstream = upstream.contiguous()
-        with _Launch(z.device) as stream:
-            _cabi.check(_cabi.load().qz_policy_loss_backward(C.byref(_struct(z, actions, legal, ctx.terms.kind)), C.byref(t), upstream.data_ptr(),
-                                                             0 if fresh else 1, grad.data_ptr(), grad.stride(0), ws.data_ptr(), size, stream))
-        return (grad,) + (None,) * 8
+        _call(z.device, _cabi.load().qz_policy_loss_backward, rows, t, upstream.data_ptr(), kept, grad.data_ptr(), z.shape[1], ws.data_ptr(), size)
+        return grad, None, None, None, None, None, None, None, None
 
 
 def _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef):
@@ -271,8 +298,17 @@ def clipped_policy_loss(logits, actions, advantages, old_logp, legal: Optional[t
     Differentiable in ``logits``; memory for their gradient is taken in the forward pass."""
     args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
     _refuse_captured_leaf(logits)
-    loss, logp, kl, entropy = _ClippedPolicyLoss.apply(*args)
-    return PolicyLoss(loss, logp.reshape(lead), kl.reshape(lead), entropy.reshape(lead))
+    if args[0].requires_grad and torch.is_grad_enabled():
+        loss, logp, kl, entropy = _ClippedPolicyLoss.apply(*args)
+    else:
+        loss, logp, kl, entropy, _, _ = _run_loss(_unit_rows(args[0]), *args[1:], False)
+    return _result(loss, logp, kl, entropy, lead)
+
+
+def _result(loss, logp, kl, entropy, lead):
+    if len(lead) != 1:
+        logp, kl, entropy = logp.reshape(lead), kl.reshape(lead), entropy.reshape(lead)
+    return PolicyLoss(loss, logp, kl, entropy)
 
 
 @torch.no_grad()
@@ -281,5 +317,5 @@ def policy_loss_and_grad(logits, actions, advantages, old_logp, legal=None, weig
     """(PolicyLoss, gradient of its loss in the logits) without the autograd graph: what a captured HIP graph records."""
     args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
     z = _unit_rows(args[0])
-    loss, logp, kl, entropy, grad = _run_loss(z, *args[1:], True)
-    return PolicyLoss(loss, logp.reshape(lead), kl.reshape(lead), entropy.reshape(lead)), grad.reshape(logits.shape)
+    loss, logp, kl, entropy, grad, _ = _run_loss(z, *args[1:], True)
+    return _result(loss, logp, kl, entropy, lead), grad.reshape(logits.shape)

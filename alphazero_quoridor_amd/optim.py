@@ -3,13 +3,15 @@
 (csrc/qz_ortho.hip: qz_orthogonalize, qz_muon_step).  There is no CPU path."""
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
+import struct
 
 import torch
 
 from . import _cabi
-from .losses import DTYPES, _gpu, _Launch
+from .losses import DTYPES, _call, _gpu
 
 
 def _matrix(t, name):
@@ -22,9 +24,19 @@ def _matrix(t, name):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _workspace(lst, count, device):
-    size = _cabi.load().qz_orthogonalize_workspace(lst, count)
-    return torch.empty(max(size, 1), dtype=torch.uint8, device=device), size
+class _List:
+    """qz_matrix[]: nine 8-byte words a matrix (the last one holds a float), written as one run of integers."""
+
+    def __init__(self, words, device):
+        self.words = array.array("q", words)
+        self.count = len(words) // 9
+        self.ptr = C.cast(self.words.buffer_info()[0], C.POINTER(_cabi.qz_matrix))
+        self.size = _cabi.load().qz_orthogonalize_workspace(self.ptr, self.count)
+        self.ws = torch.empty(max(self.size, 1), dtype=torch.uint8, device=device)
+
+
+def _float_word(v):
+    return struct.unpack("q", struct.pack("fi", v, 0))[0]
 
 
 @torch.no_grad()
@@ -37,19 +49,20 @@ def orthogonalize(update, steps=5):
     steps = int(steps)
     if not 1 <= steps <= 16:
         raise ValueError("steps = %d is not in 1 .. 16" % steps)
-    mats = [_matrix(u, "update") for u in updates]
-    outs = [torch.empty(u.shape, dtype=u.dtype, device=u.device) for u in updates]
+    outs, batches, keep = [], {}, []
     for u in updates:
+        m = _matrix(u, "update")
         if u.dtype not in DTYPES:
             raise TypeError("update: %s is not one of float32, bfloat16, float16" % u.dtype)
-    for key in dict.fromkeys((u.dtype, u.device) for u in updates):
-        lst = [(m, o) for m, o, u in zip(mats, outs, updates) if (u.dtype, u.device) == key and u.numel()]
-        if not lst:
-            continue
-        arr = (_cabi.qz_matrix * len(lst))(*[(m.shape[0], m.shape[1], m.data_ptr(), m.stride(0), o.data_ptr(), m.shape[1]) for m, o in lst])
-        ws, size = _workspace(arr, len(lst), key[1])
-        with _Launch(key[1]) as stream:
-            _cabi.check(_cabi.load().qz_orthogonalize(arr, len(lst), DTYPES[key[0]], steps, ws.data_ptr(), size, stream))
+        o = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+        outs.append(o)
+        keep.append(m)  # (may be a copy: it lives until the launches are queued)
+        rows, cols = m.shape
+        if rows and cols:
+            batches.setdefault((u.dtype, u.device), []).extend((rows, cols, m.data_ptr(), m.stride(0), o.data_ptr(), cols, 0, 0, 0))
+    for (dtype, device), words in batches.items():
+        lst = _List(words, device)
+        _call(device, _cabi.load().qz_orthogonalize, lst.ptr, lst.count, DTYPES[dtype], steps, lst.ws.data_ptr(), lst.size)
     return outs if many else outs[0]
 
 
@@ -86,43 +99,44 @@ class Muon(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         for group in self.param_groups:
-            batches = {}
+            adam, batches, changed = group["adjust_lr"] == "match_rms_adamw", {}, []
             for p in group["params"]:
-                if p.grad is None or p.numel() == 0:
+                g = p.grad
+                if g is None or p.numel() == 0:
                     continue
-                _gpu(p, "parameter")
-                if p.grad.is_sparse or p.grad.dtype not in DTYPES:
-                    raise TypeError("gradient: %s is not a dense float32, bfloat16 or float16 tensor" % p.grad.dtype)
+                if g.layout is not torch.strided or g.dtype not in DTYPES:
+                    raise TypeError("gradient: %s is not a dense float32, bfloat16 or float16 tensor" % g.dtype)
                 state = self.state[p]
-                if "momentum_buffer" not in state:
-                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
-                buf = state["momentum_buffer"]
-                if buf.shape != p.shape or buf.dtype != torch.float32 or not buf.is_contiguous() or buf.device != p.device or not p.is_contiguous():
+                buf = state.get("momentum_buffer")
+                if buf is None:
+                    _gpu(p, "parameter")
+                    buf = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                if buf.shape != p.shape or buf.dtype is not torch.float32 or p.dtype is not torch.float32 or buf.device != p.device \
+                        or not buf.is_contiguous() or not p.is_contiguous():
                     raise ValueError("a weight and its momentum must be contiguous float32 tensors of one shape and device")
-                batches.setdefault((p.grad.dtype, p.device), []).append((p, _matrix(p.grad, "gradient"), buf))
-            for (dtype, device), lst in batches.items():
-                self._batch(group, dtype, device, lst)
+                m = _matrix(g, "gradient")
+                rows, cols = m.shape
+                scale = 0.2 * math.sqrt(max(rows, cols)) if adam else math.sqrt(rows / cols) if rows > cols else 1.0
+                words, keep = batches.setdefault((g.dtype, p.device), ([], []))
+                words.extend((rows, cols, m.data_ptr(), m.stride(0), 0, 0, buf.data_ptr(), p.data_ptr(), _float_word(scale)))
+                keep.append(m)
+                changed += (p, buf)
+            for (dtype, device), (words, _) in batches.items():
+                self._batch(group, dtype, device, words)
+            if changed:
+                torch.autograd.graph.increment_version(changed)
         return loss
 
     @staticmethod
-    def _batch(group, dtype, device, lst):
+    def _batch(group, dtype, device, words):
         lr = group["lr"]
         lr_dev = lr if torch.is_tensor(lr) and lr.is_cuda else None
         if lr_dev is not None and (lr_dev.dtype != torch.float32 or lr_dev.numel() != 1 or lr_dev.device != device):
             raise ValueError("a learning rate on the GPU must be one float32 on the parameters' device")
-        adam = group["adjust_lr"] == "match_rms_adamw"
-        rows = []
-        for p, g, buf in lst:
-            m, n = g.shape
-            scale = 0.2 * math.sqrt(max(m, n)) if adam else math.sqrt(max(1.0, m / n))
-            rows.append((m, n, g.data_ptr(), g.stride(0), 0, 0, buf.data_ptr(), p.data_ptr(), scale))
-        arr = (_cabi.qz_matrix * len(rows))(*rows)
         opts = _cabi.qz_muon_opts(0.0 if lr_dev is not None else float(lr), group["momentum"], group["weight_decay"], int(group["nesterov"]),
                                   lr_dev.data_ptr() if lr_dev is not None else 0)
-        ws, size = _workspace(arr, len(rows), device)
-        with _Launch(device) as stream:
-            _cabi.check(_cabi.load().qz_muon_step(arr, len(rows), DTYPES[dtype], group["ns_steps"], C.byref(opts), ws.data_ptr(), size, stream))
-        torch.autograd.graph.increment_version([t for p, _, buf in lst for t in (p, buf)])
+        lst = _List(words, device)
+        _call(device, _cabi.load().qz_muon_step, lst.ptr, lst.count, DTYPES[dtype], group["ns_steps"], opts, lst.ws.data_ptr(), lst.size)
 
 
 class Chained:
