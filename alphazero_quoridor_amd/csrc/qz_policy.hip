@@ -90,22 +90,26 @@ __device__ __forceinline__ float chunk_get<__half>(const Raw& r, int k) {
     return (float)__builtin_bit_cast(_Float16, h);
 }
 template <typename T>
+__device__ __forceinline__ void store_full(T* at, const float* v) {
+    Raw r;
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) r.w[k] = __float_as_uint(v[k]);
+    } else if (__is_same(T, __half)) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k + 1]) << 16;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k + 1]) << 16;
+    }
+    __builtin_memcpy(at, &r, 16);
+}
+template <typename T>
 __device__ __forceinline__ void store_chunk(void* row, int64_t j0, int n, const float* v) {
     if (j0 + Elem<T>::V <= n) {
-        Raw r;
-        if (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) r.w[k] = __float_as_uint(v[k]);
-        } else if (__is_same(T, __half)) {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * k + 1]) << 16;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                r.w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k]) | (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)v[2 * k + 1]) << 16;
-        }
-        __builtin_memcpy(static_cast<T*>(row) + j0, &r, 16);
+        store_full<T>(static_cast<T*>(row) + j0, v);
     } else {
 #pragma unroll
         for (int k = 0; k < Elem<T>::V; k++)
@@ -304,34 +308,76 @@ __device__ __forceinline__ float block_sum(float v, float* sh) {
     return r;
 }
 
-// the statistics of the columns that one thread visits, online: one running (m, s, t), rescaled once per 16-byte chunk
+// ---- illegal columns as -inf, in the packed words
 template <typename T>
-__device__ __forceinline__ void stat_chunk(Stat& st, const Raw& raw, uint32_t ok) {
-    constexpr int V = Elem<T>::V;
-    float cm = NEG_INF;
-    bool bad = false;
+struct NegInf {
+    static constexpr uint32_t pair = __is_same(T, __half) ? 0xFC00FC00u : __is_same(T, float) ? 0xFF800000u : 0xFF80FF80u;
+};
+template <typename T>
+__device__ __forceinline__ Raw raw_empty() {
+    return {{NegInf<T>::pair, NegInf<T>::pair, NegInf<T>::pair, NegInf<T>::pair}};
+}
+// columns whose bit of ok is clear become -inf
+template <typename T>
+__device__ __forceinline__ void raw_mask(Raw& raw, uint32_t ok) {
 #pragma unroll
-    for (int k = 0; k < V; k++)
-        if ((ok >> k) & 1u) {
-            const float z = chunk_get<T>(raw, k);
-            cm = fmaxf(cm, z);
-            bad |= z != z;
+    for (int w = 0; w < 4; w++) {
+        if (sizeof(T) == 4) {
+            raw.w[w] = (ok >> w) & 1u ? raw.w[w] : NegInf<T>::pair;
+        } else {
+            const uint32_t keep = ((ok >> (2 * w)) & 1u ? 0x0000FFFFu : 0u) | ((ok >> (2 * w + 1)) & 1u ? 0xFFFF0000u : 0u);
+            raw.w[w] = (raw.w[w] & keep) | (NegInf<T>::pair & ~keep);
         }
-    if (bad) st.s = __builtin_nanf("");
+    }
+}
+// the same from a mask of bytes, four at a time: 0xFF in every non-zero byte, spread over its column's bits
+template <typename T>
+__device__ __forceinline__ void raw_mask_bytes(Raw& raw, const uint8_t* b) {
+    uint32_t w[2] = {0u, 0u};
+    __builtin_memcpy(w, b, Elem<T>::V);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::V / 4; i++) {
+        uint32_t t = (((w[i] & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | w[i]) & 0x80808080u;
+        t |= t - (t >> 7);
+#pragma unroll
+        for (int k = 0; k < (sizeof(T) == 4 ? 4 : 2); k++) {
+            const uint32_t keep = __builtin_amdgcn_perm(0u, t, sizeof(T) == 4 ? 0x01010101u * k : k ? 0x03030202u : 0x01010000u);
+            uint32_t& v = raw.w[sizeof(T) == 4 ? k : 2 * i + k];
+            v = (v & keep) | (NegInf<T>::pair & ~keep);
+        }
+    }
+}
+// the legal columns j0 .. j0 + V - 1 of a row, illegal and missing ones as -inf
+template <typename T>
+__device__ __forceinline__ Raw load_legal(const PolicyRows& R, const void* row, int64_t r, int64_t j0) {
+    constexpr int V = Elem<T>::V;
+    Raw raw = load_chunk<T>(row, j0, R.a);
+    if (R.legal_kind == 2 && j0 + V <= R.a) raw_mask_bytes<T>(raw, static_cast<const uint8_t*>(R.legal) + r * R.legal_ld + j0);
+    else if (R.legal_kind != 0 || j0 + V > R.a) raw_mask<T>(raw, legal_bits<V>(R, r, j0));
+    return raw;
+}
+
+// the statistics of the columns that one thread visits, online: one running (m, s, t), rescaled where a chunk brings a new maximum.
+// m starts at the lowest finite value, so that a chunk of -inf only adds exp(-inf) = 0; a NaN reaches s, which keeps it.
+constexpr float LOWEST = -3.402823466e38f;
+template <typename T>
+__device__ __forceinline__ void stat_chunk(Stat& st, const Raw& raw) {
+    constexpr int V = Elem<T>::V;
+    float cm = chunk_get<T>(raw, 0);
+#pragma unroll
+    for (int k = 1; k < V; k++) cm = fmaxf(cm, chunk_get<T>(raw, k));
     if (cm > st.m) {
-        const float d = st.m - cm, e = st.s == 0.f ? 0.f : exp2_fast(d * LOG2E);
-        st.t = e != 0.f ? (st.t + st.s * d) * e : 0.f;
-        st.s = st.s != st.s ? st.s : st.s * e;
+        const float d = fmaxf(st.m - cm, LOWEST), e = exp2_fast(d * LOG2E);
+        st.t = e != 0.f ? (st.t + st.s * d) * e : 0.f * st.t;
+        st.s *= e;
         st.m = cm;
     }
-    if (st.m == NEG_INF) return;
 #pragma unroll
-    for (int k = 0; k < V; k++)
-        if ((ok >> k) & 1u) {
-            const float x = chunk_get<T>(raw, k) - st.m, e = exp2_fast(x * LOG2E);
-            st.s += e;
-            st.t += e != 0.f ? e * x : 0.f;
-        }
+    for (int k = 0; k < V; k++) {
+        const float x = chunk_get<T>(raw, k) - st.m, e = exp2_fast(x * LOG2E);
+        st.s += e;
+        st.t += e * fmaxf(x, -1e30f);
+    }
 }
 
 // ================================================================ any width: one workgroup per row, the row read twice
@@ -340,8 +386,17 @@ constexpr int RT = 256;
 template <typename T>
 __device__ __forceinline__ Stat row_stat(const PolicyRows& R, const void* base, int64_t ld, int64_t row, float* sh) {
     const T* z = static_cast<const T*>(base) + row * ld;
-    Stat st = stat_empty();
-    for (int64_t j = (int64_t)threadIdx.x * Elem<T>::V; j < R.a; j += RT * Elem<T>::V) stat_chunk<T>(st, load_chunk<T>(z, j, R.a), legal_bits<Elem<T>::V>(R, row, j));
+    constexpr int V = Elem<T>::V, STEP = RT * V;
+    Stat st = {LOWEST, 0.f, 0.f};
+    int64_t j = (int64_t)threadIdx.x * V;
+    for (; j + 3 * STEP + V <= R.a; j += 4 * STEP) {  // four chunks' loads in flight
+        Raw r[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) r[k] = load_legal<T>(R, z, row, j + k * STEP);
+#pragma unroll
+        for (int k = 0; k < 4; k++) stat_chunk<T>(st, r[k]);
+    }
+    for (; j < R.a; j += STEP) stat_chunk<T>(st, load_legal<T>(R, z, row, j));
     return block_join<RT>(st, sh);
 }
 
@@ -436,6 +491,312 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
     }
 }
 
+// ================================================================ narrow rows: a wave per row, the row in registers
+// Bound by launch and memory latency at the sizes that boards have (13,312 rows of 140); four rows per workgroup.
+template <typename T>
+__device__ __forceinline__ float masked(const PolicyRows& R, int64_t row, const void* base, int64_t ld, int64_t j) {
+    if (j >= R.a || !legal_one(R, row, j)) return NEG_INF;
+    return Elem<T>::get(static_cast<const T*>(base) + row * ld, j);
+}
+// (m, s, t) of a row whose E values per lane are in registers (-inf: no such column, or an illegal one)
+template <int E>
+__device__ __forceinline__ Stat wave_stat(const float (&z)[E]) {
+    float m = z[0];
+#pragma unroll
+    for (int e = 1; e < E; e++) m = fmaxf(m, z[e]);
+    Stat st;
+    st.m = wave_max(m);
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const float x = z[e] - st.m, p = exp2_fast(x * LOG2E);
+        s += p;
+        t += p * fmaxf(x, -1e30f);  // (p = 0 where x is -inf)
+    }
+    st.s = wave_sum(s);
+    st.t = wave_sum(t);
+    return st;
+}
+template <typename T, int E>
+__global__ __launch_bounds__(256) void k_wave_logp(PolicyRows R, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= R.n) return;
+    float z[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) z[e] = masked<T>(R, row, R.logits, R.ld, lane + 64 * e);
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    const Stat st = wave_stat<E>(z);
+    if (lane == 0) {
+        const float ls = stat_log(st);
+        logp[row] = live ? (za - st.m) - ls : act < 0 ? 0.f : NEG_INF;
+        if (entropy) entropy[row] = live ? stat_entropy(st) : 0.f;
+        if (stats) {
+            stats[row] = live ? st.m : 0.f;
+            stats[R.n + row] = live ? ls : 0.f;
+        }
+    }
+}
+template <typename T, int E>
+__global__ __launch_bounds__(256) void k_wave_loss(PolicyRows R, PolicyTerms P, PolicyOut O) {
+    const float scale = O.scale ? *O.scale : 1.f;
+    if (O.only_if_scaled && scale == 1.f) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= R.n) return;
+    const bool has_q = P.ref_logits != nullptr;
+    float z[E], zq[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        z[e] = masked<T>(R, row, R.logits, R.ld, lane + 64 * e);
+        zq[e] = has_q ? masked<T>(R, row, P.ref_logits, P.ref_ld, lane + 64 * e) : NEG_INF;
+    }
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    RowOut o = {act < 0 ? 0.f : NEG_INF, 0.f, {}};
+    float kl = 0.f, h = 0.f;
+    if (live) {
+        const Stat st = wave_stat<E>(z);
+        const Stat sq = has_q ? wave_stat<E>(zq) : Stat{0.f, 1.f, 0.f};
+        o = row_terms(P, row, act, za, st, sq, scale);
+        h = o.g.h;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            // an illegal column is -inf in both: p = q = 0, its terms 0 (an infinite coefficient is kept out below)
+            const float d = column(o.g, has_q, z[e], zq[e], lane + 64 * e, kl);
+            z[e] = z[e] == NEG_INF && zq[e] == NEG_INF ? 0.f : d;
+        }
+        kl = has_q ? wave_sum(kl) : kl_taken(P, row, o.logp);
+    }
+    if (O.grad) {
+        T* out = static_cast<T*>(O.grad) + row * O.ld_grad;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (lane + 64 * e < R.a) Elem<T>::put(out, lane + 64 * e, live ? z[e] : 0.f);
+    }
+    if (lane == 0 && O.parts) {
+        const float w = P.weights ? P.weights[row] : P.default_weight;
+        O.logp[row] = o.logp;
+        O.kl[row] = live ? kl : 0.f;
+        O.entropy[row] = h;
+        O.parts[row] = (double)o.loss + (has_q && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+    }
+}
+
+// ================================================================ wide rows: a workgroup per row, the row in registers
+// One pass over memory: logits (and the frozen policy's) are read once, into registers as they are stored, illegal columns replaced by
+// -inf on the way; then the maximum, the sums and the gradient come from the registers.  Bound by memory where there is one input, by
+// vector instructions (~50 per column with two inputs) close behind it otherwise; two workgroups of 512 share a CU, so that one's
+// arithmetic covers the other's loads.
+template <typename T, int CH>
+__device__ __forceinline__ float chunks_max(const Raw (&z)[CH]) {
+    float m = NEG_INF;
+#pragma unroll
+    for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int k = 0; k < Elem<T>::V; k++) m = fmaxf(m, chunk_get<T>(z[c], k));
+    return m;
+}
+// The compiler must not keep the unpacked values of one pass for the next (twice the registers, and spills): to it, the packed ones
+// change between the passes.
+template <int CH>
+__device__ __forceinline__ void forget(Raw (&z)[CH]) {
+#pragma unroll
+    for (int c = 0; c < CH; c++) asm volatile("" : "+v"(z[c].w[0]), "+v"(z[c].w[1]), "+v"(z[c].w[2]), "+v"(z[c].w[3]));
+}
+template <int NT>
+__device__ __forceinline__ void block_max2(float& a, float& b, float* sh) {
+    a = wave_max(a);
+    b = wave_max(b);
+    if ((threadIdx.x & 63) == 0) {
+        sh[threadIdx.x >> 6] = a;
+        sh[16 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        a = fmaxf(a, sh[w]);
+        b = fmaxf(b, sh[16 + w]);
+    }
+}
+template <int NT>
+__device__ __forceinline__ void block_sum3(float& a, float& b, float& c, float* sh) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    c = wave_sum(c);
+    if ((threadIdx.x & 63) == 0) {
+        sh[threadIdx.x >> 6] = a;
+        sh[16 + (threadIdx.x >> 6)] = b;
+        sh[32 + (threadIdx.x >> 6)] = c;
+    }
+    __syncthreads();
+    a = b = c = 0.f;
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        a += sh[w];
+        b += sh[16 + w];
+        c += sh[32 + w];
+    }
+}
+// One column without branches, for rows whose coefficients are finite: the same values as column().  -inf in both inputs (an illegal
+// column) gives 0 and no term of KL; x is held below 1e30 so that q = 0 gives the term p and not 0 inf.
+struct FastCoef {
+    float m, ls, mq, lsq, c, eta, eh, beta, shift;  // eh = eta h - c, shift = ls - lsq
+};
+template <bool HAS_Q>
+__device__ __forceinline__ float column_fast(const FastCoef& g, float z, float zq, float& kl) {
+    const float dz = z - g.m, lp = dz - g.ls, p = exp2_fast(lp * LOG2E);
+    float d = p * (g.eta * fmaxf(lp, -1e30f) + g.eh);
+    if (HAS_Q) {
+        const float dq = zq - g.mq, q = exp2_fast((dq - g.lsq) * LOG2E), x = fminf((dz - dq) - g.shift, 1e30f), pq = p - q;
+        float r = 1.f / 720.f;
+        r = r * x + 1.f / 120.f;
+        r = r * x + 1.f / 24.f;
+        r = r * x + 1.f / 6.f;
+        r = r * x + 0.5f;
+        const float qx = q * x, near = qx * (x * r), far = pq - qx;
+        kl += fabsf(x) < 0.25f ? near : far;
+        d += g.beta * pq;
+    }
+    return d;
+}
+// a row with an infinite or NaN coefficient: its gradient column by column from memory
+template <typename T, int NT>
+__device__ __forceinline__ float row_gradient_slow(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, int64_t row, const Coef& g) {
+    float kl = 0.f;
+    const bool has_q = P.ref_logits != nullptr;
+#pragma unroll 1
+    for (int64_t j = threadIdx.x; j < R.a; j += NT) {
+        float d = 0.f;
+        if (legal_one(R, row, j))
+            d = column(g, has_q, Elem<T>::get(static_cast<const T*>(R.logits) + row * R.ld, j), has_q ? Elem<T>::get(static_cast<const T*>(P.ref_logits) + row * P.ref_ld, j) : 0.f, j, kl);
+        if (O.grad) Elem<T>::put(static_cast<T*>(O.grad) + row * O.ld_grad, j, d);
+    }
+    return kl;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+
+// A thread holds CH chunks of 16 bytes, and the first few threads one column each of what is left over of the row.
+template <typename T, int NT, int CH, bool HAS_Q, bool MASK>
+__global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P, PolicyOut O) {
+    constexpr int V = Elem<T>::V;
+    __shared__ float sh[3][48];
+    const float scale = O.scale ? *O.scale : 1.f;
+    if (O.only_if_scaled && scale == 1.f) return;
+    const int64_t row = blockIdx.x;
+    const T* zrow = static_cast<const T*>(R.logits) + row * R.ld;
+    const T* qrow = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
+    const int j0 = threadIdx.x * V, full = R.a / V * V, jt = full + threadIdx.x;
+    Raw z[CH], q[HAS_Q ? CH : 1] = {};
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+        z[c] = raw_empty<T>();
+        if (HAS_Q) q[c] = raw_empty<T>();
+        const int j = j0 + c * NT * V;
+        if (j < full) {
+            __builtin_memcpy(&z[c], zrow + j, 16);
+            if (HAS_Q) __builtin_memcpy(&q[c], qrow + j, 16);
+        }
+    }
+    if (MASK && R.legal_kind == 2) {
+        const uint8_t* b = static_cast<const uint8_t*>(R.legal) + row * R.legal_ld;
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int j = j0 + c * NT * V;
+            if (j < full) {
+                raw_mask_bytes<T>(z[c], b + j);
+                if (HAS_Q) raw_mask_bytes<T>(q[c], b + j);
+            }
+        }
+    } else if (MASK) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            const int j = j0 + c * NT * V;
+            if (j < full) {
+                const uint32_t ok = legal_bits<V>(R, row, j);
+                raw_mask<T>(z[c], ok);
+                if (HAS_Q) raw_mask<T>(q[c], ok);
+            }
+        }
+    }
+    const float zt = masked<T>(R, row, R.logits, R.ld, jt), qt = HAS_Q ? masked<T>(R, row, P.ref_logits, P.ref_ld, jt) : NEG_INF;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    T* out = static_cast<T*>(O.grad) + row * O.ld_grad;
+    RowOut o = {act < 0 ? 0.f : NEG_INF, 0.f, {}};
+    float kl = 0.f, h = 0.f;
+    if (live) {
+        float m = fmaxf(chunks_max<T, CH>(z), zt), mq = 0.f;
+        if (HAS_Q) mq = fmaxf(chunks_max<T, HAS_Q ? CH : 1>(q), qt);
+        block_max2<NT>(m, mq, sh[0]);
+        forget(z);
+        forget(q);
+        // sums in powers of two: y = (z - m) log2 e; t is turned back to natural units at the end
+        float s = 0.f, t = 0.f, sq = 0.f;
+        auto add = [&](float v, float u) {
+            const float y = (v - m) * LOG2E, e = exp2_fast(y);
+            s += e;
+            t += e * fmaxf(y, -1e30f);
+            if (HAS_Q) sq += exp2_fast((u - mq) * LOG2E);
+        };
+        add(zt, qt);
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+#pragma unroll
+            for (int k = 0; k < V; k++) add(chunk_get<T>(z[c], k), HAS_Q ? chunk_get<T>(q[c], k) : 0.f);
+            __builtin_amdgcn_sched_barrier(0);  // (a chunk at a time: interleaved further, the values in between spill)
+        }
+        block_sum3<NT>(s, t, sq, sh[1]);
+        forget(z);
+        forget(q);
+        o = row_terms(P, row, act, za, Stat{m, s, t * LN2}, HAS_Q ? Stat{mq, sq, 0.f} : Stat{0.f, 1.f, 0.f}, scale);
+        h = o.g.h;
+        const FastCoef g = {o.g.m, o.g.ls, o.g.mq, o.g.lsq, o.g.c, o.g.eta, o.g.eta * h - o.g.c, o.g.beta, o.g.ls - o.g.lsq};
+        if (!finite(g.eh) || !finite(g.eta) || !finite(g.c) || !finite(g.beta) || !finite(g.shift) || !finite(g.m)) {
+            kl = row_gradient_slow<T, NT>(R, P, O, row, o.g);
+        } else if (O.grad || HAS_Q) {
+            const int a32 = (int)act;
+            const float dt = column_fast<HAS_Q>(g, zt, qt, kl) + (jt == a32 ? g.c : 0.f);
+            if (O.grad && jt < R.a) Elem<T>::put(out, jt, dt);
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                const int j = j0 + c * NT * V;
+                float d[V];
+#pragma unroll
+                for (int k = 0; k < V; k++) d[k] = column_fast<HAS_Q>(g, chunk_get<T>(z[c], k), HAS_Q ? chunk_get<T>(q[c], k) : 0.f, kl);
+                asm volatile("" : "+v"(kl));  // (or the terms of KL are put off to the last chunk, with all their inputs kept)
+                if ((unsigned)(a32 - j) < (unsigned)V) {
+#pragma unroll
+                    for (int k = 0; k < V; k++) d[k] += a32 - j == k ? g.c : 0.f;
+                }
+                if (O.grad && j < full) store_full<T>(out + j, d);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (HAS_Q) {
+            float a = 0.f, b = 0.f;
+            block_sum3<NT>(kl, a, b, sh[2]);
+        } else {
+            kl = kl_taken(P, row, o.logp);
+        }
+    } else if (O.grad) {
+        const float zero[V] = {};
+        for (int j = j0; j < full; j += NT * V) store_full<T>(out + j, zero);
+        if (jt < R.a) Elem<T>::put(out, jt, 0.f);
+    }
+    if (threadIdx.x == 0 && O.parts) {
+        const float w = P.weights ? P.weights[row] : P.default_weight;
+        O.logp[row] = o.logp;
+        O.kl[row] = live ? kl : 0.f;
+        O.entropy[row] = h;
+        O.parts[row] = (double)o.loss + (HAS_Q && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+    }
+}
+
 __global__ __launch_bounds__(1024) void k_sum_parts(const double* __restrict__ parts, int64_t n, float* __restrict__ loss) {
     __shared__ double sh[1024];
     double s = 0.0;
@@ -458,11 +819,46 @@ __global__ __launch_bounds__(1024) void k_sum_parts(const double* __restrict__ p
         default: { using T = __half; CALL; break; }                                       \
     }
 
+namespace {
+// rows of up to 1,024 columns stay with one wave (16 registers of values per lane); 140 columns take 3
+constexpr int WAVE_WIDEST = 1024;
+#define BY_WIDTH(a, CALL)                                   \
+    if ((a) <= 64) { constexpr int E = 1; CALL; }           \
+    else if ((a) <= 192) { constexpr int E = 3; CALL; }     \
+    else if ((a) <= 512) { constexpr int E = 8; CALL; }     \
+    else { constexpr int E = 16; CALL; }
+
+template <typename T, int NT, int CH>
+void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
+    const dim3 grid((unsigned)R.n), block(NT);
+    if (P.ref_logits && R.legal_kind) hipLaunchKernelGGL((k_row_loss<T, NT, CH, true, true>), grid, block, 0, s, R, P, O);
+    else if (P.ref_logits) hipLaunchKernelGGL((k_row_loss<T, NT, CH, true, false>), grid, block, 0, s, R, P, O);
+    else if (R.legal_kind) hipLaunchKernelGGL((k_row_loss<T, NT, CH, false, true>), grid, block, 0, s, R, P, O);
+    else hipLaunchKernelGGL((k_row_loss<T, NT, CH, false, false>), grid, block, 0, s, R, P, O);
+}
+// the smallest workgroup whose registers hold the row; past 1,024 threads of 8 chunks the row is read twice
+template <typename T>
+void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
+    const int chunks = (R.a + Elem<T>::V - 1) / Elem<T>::V;
+    if (chunks <= 256) row_loss<T, 256, 1>(R, P, O, s);
+    else if (chunks <= 512) row_loss<T, 256, 2>(R, P, O, s);
+    else if (chunks <= 1024) row_loss<T, 256, 4>(R, P, O, s);
+    else if (chunks <= 2048) row_loss<T, 512, 4>(R, P, O, s);
+    else if (chunks <= 4096) row_loss<T, 512, 8>(R, P, O, s);
+    else if (chunks <= 8192) row_loss<T, 1024, 8>(R, P, O, s);
+    else hipLaunchKernelGGL((k_policy_loss<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, P, O);
+}
+}  // namespace
+
 namespace qzl {
 int64_t policy_workspace_bytes(int64_t n, int a) { return n * (int64_t)sizeof(double); }
 
 hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void*, hipStream_t s) {
     if (R.n <= 0) return hipSuccess;
+    if (R.a <= WAVE_WIDEST) {
+        BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_logp<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats)));
+        return hipGetLastError();
+    }
     BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, logp, entropy, stats));
     return hipGetLastError();
 }
@@ -474,7 +870,13 @@ hipError_t action_logp_backward(const PolicyRows& R, const float* stats, const f
 }
 hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, float* loss, void* ws, hipStream_t s) {
     O.parts = loss ? static_cast<double*>(ws) : nullptr;
-    if (R.n > 0) BY_TYPE(R.dtype, hipLaunchKernelGGL((k_policy_loss<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, P, O));
+    if (R.n > 0) {
+        if (R.a <= WAVE_WIDEST) {
+            BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_loss<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, P, O)));
+        } else {
+            BY_TYPE(R.dtype, wide_loss<T>(R, P, O, s));
+        }
+    }
     if (loss) hipLaunchKernelGGL(k_sum_parts, dim3(1), dim3(1024), 0, s, O.parts, R.n, loss);
     return hipGetLastError();
 }
