@@ -381,26 +381,26 @@ __device__ __forceinline__ void stat_chunk(Stat& st, const Raw& raw) {
 }
 
 // ================================================================ any width: one workgroup per row, the row read twice
-constexpr int RT = 256;
 
-template <typename T>
-__device__ __forceinline__ Stat row_stat(const PolicyRows& R, const void* base, int64_t ld, int64_t row, float* sh) {
+// j0, j1: the columns of this workgroup (j0 a multiple of a chunk)
+template <typename T, int RT>
+__device__ __forceinline__ Stat row_stat(const PolicyRows& R, const void* base, int64_t ld, int64_t row, int64_t j0, int64_t j1, float* sh) {
     const T* z = static_cast<const T*>(base) + row * ld;
     constexpr int V = Elem<T>::V, STEP = RT * V;
     Stat st = {LOWEST, 0.f, 0.f};
-    int64_t j = (int64_t)threadIdx.x * V;
-    for (; j + 3 * STEP + V <= R.a; j += 4 * STEP) {  // four chunks' loads in flight
+    int64_t j = j0 + (int64_t)threadIdx.x * V;
+    for (; j + 3 * STEP + V <= j1; j += 4 * STEP) {  // four chunks' loads in flight
         Raw r[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) r[k] = load_legal<T>(R, z, row, j + k * STEP);
 #pragma unroll
         for (int k = 0; k < 4; k++) stat_chunk<T>(st, r[k]);
     }
-    for (; j < R.a; j += STEP) stat_chunk<T>(st, load_legal<T>(R, z, row, j));
+    for (; j < j1; j += STEP) stat_chunk<T>(st, load_legal<T>(R, z, row, j));
     return block_join<RT>(st, sh);
 }
 
-template <typename T>
+template <typename T, int RT>
 __global__ __launch_bounds__(RT) void k_action_logp(PolicyRows R, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
     __shared__ float sh[3 * RT / 64];
     const int64_t row = blockIdx.x;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(RT) void k_action_logp(PolicyRows R, float* __restr
     float za;
     const bool live = row_live<T>(R, row, act, za);
     Stat st = stat_empty();
-    if (live) st = row_stat<T>(R, R.logits, R.ld, row, sh);
+    if (live) st = row_stat<T, RT>(R, R.logits, R.ld, row, 0, R.a, sh);
     if (threadIdx.x == 0) {
         const float ls = stat_log(st);
         logp[row] = live ? (za - st.m) - ls : act < 0 ? 0.f : NEG_INF;
@@ -420,8 +420,9 @@ __global__ __launch_bounds__(RT) void k_action_logp(PolicyRows R, float* __restr
     }
 }
 
+constexpr int BT = 256;
 template <typename T>
-__global__ __launch_bounds__(RT) void k_action_logp_backward(PolicyRows R, const float* __restrict__ stats, const float* __restrict__ entropy,
+__global__ __launch_bounds__(BT) void k_action_logp_backward(PolicyRows R, const float* __restrict__ stats, const float* __restrict__ entropy,
                                                              const float* __restrict__ dlogp, const float* __restrict__ dentropy, void* __restrict__ grad,
                                                              int64_t ld_grad) {
     constexpr int V = Elem<T>::V;
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(RT) void k_action_logp_backward(PolicyRows R, const
     const T* z = static_cast<const T*>(R.logits) + row * R.ld;
     T* out = static_cast<T*>(grad) + row * ld_grad;
     const Coef g = {stats[row], stats[R.n + row], entropy ? entropy[row] : 0.f, dlogp ? dlogp[row] : 0.f, 0.f, dentropy ? -dentropy[row] : 0.f, 0.f, 0.f, act, true};
-    for (int64_t j = ((int64_t)blockIdx.y * RT + threadIdx.x) * V; j < R.a; j += (int64_t)gridDim.y * RT * V) {
+    for (int64_t j = ((int64_t)blockIdx.y * BT + threadIdx.x) * V; j < R.a; j += (int64_t)gridDim.y * BT * V) {
         const uint32_t ok = live ? legal_bits<V>(R, row, j) : 0u;
         const Raw raw = load_chunk<T>(z, j, R.a);
         float d[V], kl = 0.f;
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(RT) void k_action_logp_backward(PolicyRows R, const
     }
 }
 
-template <typename T>
+template <typename T, int RT>
 __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P, PolicyOut O) {
     constexpr int V = Elem<T>::V;
     __shared__ float sh[3 * RT / 64];
@@ -457,9 +458,9 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
     RowOut o = {act < 0 ? 0.f : NEG_INF, 0.f, {}};
     float h = 0.f;
     if (live) {
-        const Stat st = row_stat<T>(R, R.logits, R.ld, row, sh);
+        const Stat st = row_stat<T, RT>(R, R.logits, R.ld, row, 0, R.a, sh);
         const bool has_q = P.ref_logits != nullptr;
-        const Stat sq = has_q ? row_stat<T>(R, P.ref_logits, P.ref_ld, row, sh) : Stat{0.f, 1.f, 0.f};
+        const Stat sq = has_q ? row_stat<T, RT>(R, P.ref_logits, P.ref_ld, row, 0, R.a, sh) : Stat{0.f, 1.f, 0.f};
         h = stat_entropy(st);
         o = row_terms(P, row, act, za, st, sq, scale);
         const T* z = static_cast<const T*>(R.logits) + row * R.ld;
@@ -489,6 +490,121 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
         O.entropy[row] = h;
         O.parts[row] = (double)o.loss + (P.ref_logits && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
     }
+}
+
+// ================================================================ few wide rows: several workgroups per row
+// A CU alone draws some 40 GB/s from memory, so a row of 131,072 columns takes 10 us and more; S workgroups take pieces of it.  First
+// launch: every piece's (m, s, t) of both inputs.  Second: each workgroup joins the row's S triples (in order, so that all agree bit
+// for bit), and does its piece of the gradient and of KL.  Third: one workgroup sums KL and the loss.
+constexpr int ST = 256, MAX_SPLIT = 64;
+struct Split {
+    int32_t s;       // pieces per row
+    int32_t piece;   // columns of one, a multiple of ST chunks
+    float* stats;    // [n][2][s][3]: logits, frozen policy
+    float* kl;       // [n][s]
+    float* coef;     // [n]: w kl_coef of rows with a KL over logits, else 0
+};
+template <typename T>
+__global__ __launch_bounds__(ST) void k_split_stats(PolicyRows R, PolicyTerms P, Split S, const float* scale, int only_if_scaled) {
+    __shared__ float sh[3 * ST / 64];
+    if (only_if_scaled && *scale == 1.f) return;
+    const int64_t row = blockIdx.y, j0 = (int64_t)blockIdx.x * S.piece, j1 = j0 + S.piece < R.a ? j0 + S.piece : R.a;
+    for (int k = 0; k < (P.ref_logits ? 2 : 1); k++) {
+        const Stat st = k == 0 ? row_stat<T, ST>(R, R.logits, R.ld, row, j0, j1, sh) : row_stat<T, ST>(R, P.ref_logits, P.ref_ld, row, j0, j1, sh);
+        float* out = S.stats + ((row * 2 + k) * S.s + blockIdx.x) * 3;
+        if (threadIdx.x < 3) out[threadIdx.x] = threadIdx.x == 0 ? st.m : threadIdx.x == 1 ? st.s : st.t;
+    }
+}
+__device__ __forceinline__ Stat split_join(const Split& S, int64_t row, int k) {
+    const int lane = threadIdx.x & 63;
+    const float* in = S.stats + ((row * 2 + k) * S.s + lane) * 3;
+    return wave_join(lane < S.s ? Stat{in[0], in[1], in[2]} : Stat{LOWEST, 0.f, 0.f});
+}
+template <typename T>
+__global__ __launch_bounds__(64) void k_split_logp(PolicyRows R, Split S, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
+    const int64_t row = blockIdx.x;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za);
+    const Stat st = split_join(S, row, 0);
+    if (threadIdx.x == 0) {
+        const float ls = stat_log(st);
+        logp[row] = live ? (za - st.m) - ls : act < 0 ? 0.f : NEG_INF;
+        if (entropy) entropy[row] = live ? stat_entropy(st) : 0.f;
+        if (stats) {
+            stats[row] = live ? st.m : 0.f;
+            stats[R.n + row] = live ? ls : 0.f;
+        }
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(ST) void k_split_loss(PolicyRows R, PolicyTerms P, PolicyOut O, Split S) {
+    constexpr int V = Elem<T>::V;
+    __shared__ float sh[ST / 64];
+    const float scale = O.scale ? *O.scale : 1.f;
+    if (O.only_if_scaled && scale == 1.f) return;
+    const int64_t row = blockIdx.y, j0 = (int64_t)blockIdx.x * S.piece, j1 = j0 + S.piece < R.a ? j0 + S.piece : R.a;
+    int64_t act;
+    float za;
+    const bool live = row_live<T>(R, row, act, za), has_q = P.ref_logits != nullptr;
+    T* out = static_cast<T*>(O.grad) + row * O.ld_grad;
+    RowOut o = {act < 0 ? 0.f : NEG_INF, 0.f, {}};
+    float kl = 0.f;
+    if (live) {
+        o = row_terms(P, row, act, za, split_join(S, row, 0), has_q ? split_join(S, row, 1) : Stat{0.f, 1.f, 0.f}, scale);
+        const T* z = static_cast<const T*>(R.logits) + row * R.ld;
+        const T* zq = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
+        if (O.grad || has_q) {
+            for (int64_t j = j0 + (int64_t)threadIdx.x * V; j < j1; j += ST * V) {
+                const uint32_t ok = legal_bits<V>(R, row, j);
+                const Raw raw = load_chunk<T>(z, j, R.a);
+                Raw rq = {};
+                if (has_q) rq = load_chunk<T>(zq, j, R.a);
+                float d[V];
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    d[k] = (ok >> k) & 1u ? column(o.g, has_q, chunk_get<T>(raw, k), has_q ? chunk_get<T>(rq, k) : 0.f, j + k, kl) : 0.f;
+                if (O.grad) store_chunk<T>(out, j, R.a, d);
+            }
+        }
+        if (has_q) kl = block_sum<ST>(kl, sh);
+    } else if (O.grad) {
+        const float zero[V] = {};
+        for (int64_t j = j0 + (int64_t)threadIdx.x * V; j < j1; j += ST * V) store_chunk<T>(out, j, R.a, zero);
+    }
+    if (threadIdx.x == 0 && O.parts) {
+        S.kl[row * S.s + blockIdx.x] = kl;
+        if (blockIdx.x == 0) {
+            const float w = P.weights ? P.weights[row] : P.default_weight;
+            O.logp[row] = o.logp;
+            O.entropy[row] = live ? o.g.h : 0.f;
+            O.kl[row] = live && !has_q ? kl_taken(P, row, o.logp) : 0.f;
+            O.parts[row] = (double)o.loss;
+            S.coef[row] = has_q && live ? w * P.kl_coef : 0.f;
+        }
+    }
+}
+// rows' KL from their pieces, and the loss (n <= FEW_ROWS)
+__global__ __launch_bounds__(256) void k_split_finish(PolicyOut O, Split S, int n, int has_q, float* __restrict__ loss) {
+    __shared__ double sh[256];
+    double total = 0.0;
+    for (int row = threadIdx.x; row < n; row += 256) {
+        double part = O.parts[row];
+        if (has_q) {
+            float kl = 0.f;
+            for (int p = 0; p < S.s; p++) kl += S.kl[(int64_t)row * S.s + p];
+            O.kl[row] = kl;
+            if (S.coef[row] != 0.f) part += (double)S.coef[row] * kl;
+        }
+        total += part;
+    }
+    sh[threadIdx.x] = total;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = (float)sh[0];
 }
 
 // ================================================================ narrow rows: a wave per row, the row in registers
@@ -812,21 +928,21 @@ __global__ __launch_bounds__(1024) void k_sum_parts(const double* __restrict__ p
 
 }  // namespace
 
-#define BY_TYPE(dtype, CALL)                                                              \
-    switch (dtype) {                                                                      \
-        case 0: { using T = float; CALL; break; }                                         \
-        case 1: { using T = __hip_bfloat16; CALL; break; }                                \
-        default: { using T = __half; CALL; break; }                                       \
+#define BY_TYPE(dtype, ...)                                        \
+    switch (dtype) {                                               \
+        case 0: { using T = float; __VA_ARGS__; break; }           \
+        case 1: { using T = __hip_bfloat16; __VA_ARGS__; break; }  \
+        default: { using T = __half; __VA_ARGS__; break; }         \
     }
 
 namespace {
 // rows of up to 1,024 columns stay with one wave (16 registers of values per lane); 140 columns take 3
 constexpr int WAVE_WIDEST = 1024;
-#define BY_WIDTH(a, CALL)                                   \
-    if ((a) <= 64) { constexpr int E = 1; CALL; }           \
-    else if ((a) <= 192) { constexpr int E = 3; CALL; }     \
-    else if ((a) <= 512) { constexpr int E = 8; CALL; }     \
-    else { constexpr int E = 16; CALL; }
+#define BY_WIDTH(a, ...)                                    \
+    if ((a) <= 64) { constexpr int E = 1; __VA_ARGS__; }           \
+    else if ((a) <= 192) { constexpr int E = 3; __VA_ARGS__; }     \
+    else if ((a) <= 512) { constexpr int E = 8; __VA_ARGS__; }     \
+    else { constexpr int E = 16; __VA_ARGS__; }
 
 template <typename T, int NT, int CH>
 void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
@@ -846,26 +962,56 @@ void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hi
     else if (chunks <= 2048) row_loss<T, 512, 4>(R, P, O, s);
     else if (chunks <= 4096) row_loss<T, 512, 8>(R, P, O, s);
     else if (chunks <= 8192) row_loss<T, 1024, 8>(R, P, O, s);
-    else hipLaunchKernelGGL((k_policy_loss<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, P, O);
+    else if (R.n <= 1024) hipLaunchKernelGGL((k_policy_loss<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
+    else hipLaunchKernelGGL((k_policy_loss<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, P, O);
+}
+}  // namespace
+
+namespace {
+// Rows are split where a workgroup each would leave most CUs idle and a row is long enough to be worth three launches.
+constexpr int FEW_ROWS = 64, SPLIT_WIDTH = 32768;
+bool few_wide(int64_t n, int a) { return n <= FEW_ROWS && a >= SPLIT_WIDTH; }
+Split make_split(int64_t n, int a, int v, void* ws) {
+    Split S;
+    const int unit = ST * v;  // columns that one pass of a workgroup covers
+    int pieces = (int)(256 / n);
+    if (pieces > MAX_SPLIT) pieces = MAX_SPLIT;
+    if (pieces < 1) pieces = 1;
+    S.piece = (a + pieces - 1) / pieces;
+    S.piece = (S.piece + unit - 1) / unit * unit;
+    S.s = (a + S.piece - 1) / S.piece;
+    S.stats = reinterpret_cast<float*>(static_cast<char*>(ws) + n * 8);
+    S.kl = S.stats + n * 2 * MAX_SPLIT * 3;
+    S.coef = S.kl + n * MAX_SPLIT;
+    return S;
 }
 }  // namespace
 
 namespace qzl {
-int64_t policy_workspace_bytes(int64_t n, int a) { return n * (int64_t)sizeof(double); }
+int64_t policy_workspace_bytes(int64_t n, int a) { return n * 8 + (few_wide(n, a) ? n * 4 * (7 * MAX_SPLIT + 1) : 0); }
 
-hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void*, hipStream_t s) {
+hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void* ws, hipStream_t s) {
     if (R.n <= 0) return hipSuccess;
     if (R.a <= WAVE_WIDEST) {
         BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_logp<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats)));
-        return hipGetLastError();
+    } else if (few_wide(R.n, R.a)) {
+        const PolicyTerms none = {};
+        BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws);
+                hipLaunchKernelGGL((k_split_stats<T>), dim3(S.s, (unsigned)R.n), dim3(ST), 0, s, R, none, S, nullptr, 0);
+                hipLaunchKernelGGL((k_split_logp<T>), dim3((unsigned)R.n), dim3(64), 0, s, R, S, logp, entropy, stats));
+    } else if (R.n <= 1024) {  // up to four rows per CU: more waves on each
+        BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, logp, entropy, stats));
+    } else {
+        BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, logp, entropy, stats));
     }
-    BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, logp, entropy, stats));
     return hipGetLastError();
 }
 hipError_t action_logp_backward(const PolicyRows& R, const float* stats, const float* entropy, const float* dlogp, const float* dentropy, void* grad,
                                 int64_t ld_grad, hipStream_t s) {
     if (R.n <= 0) return hipSuccess;
-    BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp_backward<T>), dim3((unsigned)R.n), dim3(RT), 0, s, R, stats, entropy, dlogp, dentropy, grad, ld_grad));
+    // few rows: several workgroups for each, up to one per pass over BT chunks
+    BY_TYPE(R.dtype, const int most = (R.a + BT * Elem<T>::V - 1) / (BT * Elem<T>::V); int y = (int)((1024 + R.n - 1) / R.n); y = y < most ? y : most;
+            hipLaunchKernelGGL((k_action_logp_backward<T>), dim3((unsigned)R.n, y), dim3(BT), 0, s, R, stats, entropy, dlogp, dentropy, grad, ld_grad));
     return hipGetLastError();
 }
 hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, float* loss, void* ws, hipStream_t s) {
@@ -873,6 +1019,12 @@ hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, f
     if (R.n > 0) {
         if (R.a <= WAVE_WIDEST) {
             BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_loss<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, P, O)));
+        } else if (few_wide(R.n, R.a)) {
+            BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws); const dim3 grid(S.s, (unsigned)R.n);
+                    hipLaunchKernelGGL((k_split_stats<T>), grid, dim3(ST), 0, s, R, P, S, O.scale, O.only_if_scaled);
+                    hipLaunchKernelGGL((k_split_loss<T>), grid, dim3(ST), 0, s, R, P, O, S);
+                    if (loss) hipLaunchKernelGGL(k_split_finish, dim3(1), dim3(256), 0, s, O, S, (int)R.n, P.ref_logits != nullptr, loss));
+            return hipGetLastError();
         } else {
             BY_TYPE(R.dtype, wide_loss<T>(R, P, O, s));
         }

@@ -19,9 +19,7 @@ TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def pack(legal):
     n, a = legal.shape
-    w = torch.zeros((n, (a + 31) // 32), dtype=torch.int64)
-    for j in range(a):
-        w[:, j // 32] |= legal[:, j].long() << (j % 32)
+    w = (torch.nn.functional.pad(legal, (0, -a % 32)).view(n, -1, 32).long() << torch.arange(32)).sum(2)
     return torch.where(w >= 1 << 31, w - (1 << 32), w).to(torch.int32)
 
 
@@ -96,6 +94,12 @@ def close(got, want, tol, what):
     assert not torch.isnan(d).any(), what
     worst = (d - tol).max() if d.numel() else torch.tensor(-1.0)
     assert worst <= 0, "%s: off by %.3g past the tolerance (largest error %.3g)" % (what, float(worst), float(d.max()))
+
+
+def stored(want, dtype):
+    """A value past a type's largest one by half a step or more is rounded to infinity (float16: 65,520)."""
+    edge = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4)
+    return torch.where(want.abs() >= edge, torch.full_like(want, math.inf) * torch.sign(want), want)
 
 
 def grad_tolerance(e, dtype):
@@ -179,6 +183,39 @@ def test_action_logp_and_its_gradient(gpu_device, a, dtype):
         z3 = dev["z"].clone().requires_grad_(True)
         losses.action_logp(z3, dev["actions"], legal=legal, entropy=True)[0].sum().backward()
         assert torch.equal(z2.grad, z3.grad)
+
+
+@pytest.mark.parametrize("n,a,dtype", ((70, 66003, torch.bfloat16), (70, 66003, torch.float32), (65, 33001, torch.float16), (65, 33001, torch.float32), (64, 131072, torch.bfloat16),
+                                       (1, 131071, torch.float32), (1030, 1500, torch.bfloat16), (1030, 8200, torch.float32)), ids=str)
+def test_many_and_few_wide_rows(gpu_device, n, a, dtype):
+    """The forms that go by the number of rows as well: rows past the registers, few rows split over workgroups, many wide ones."""
+    from alphazero_quoridor_amd import losses
+
+    d = make(n, a, dtype, n + a)
+    if n > 2:
+        d["actions"][1], d["legal"][2] = -1, False
+    dev = {key: v.to(gpu_device) for key, v in d.items()}
+    for kind, kl in (("bits", "full"), ("none", "taken")):
+        e = definition(d, kind != "none", kl, (0.2, 0.2), 0.05, 0.02)
+        legal = pack(d["legal"]).to(gpu_device) if kind == "bits" else None
+        kw = dict(ref_logits=dev["ref"]) if kl == "full" else dict(ref_logp=dev["ref_logp"])
+        out, grad = losses.policy_loss_and_grad(dev["z"], dev["actions"], dev["adv"], dev["old"], legal=legal, weights=dev["w"], kl_coef=0.05, entropy_coef=0.02, **kw)
+        for name in ("loss", "logp", "entropy", "kl"):
+            close(getattr(out, name), e[name], e[name + "_tol"], "%s %s" % (kind, name))
+        close(grad, stored(e["grad"], dtype), grad_tolerance(e, dtype), "%s grad" % kind)
+        z = dev["z"].clone().requires_grad_(True)
+        logp, ent = losses.action_logp(z, dev["actions"], legal=legal, entropy=True)
+        close(logp.detach(), e["logp"], e["logp_tol"], "%s action_logp" % kind)
+        close(ent.detach(), e["entropy"], e["entropy_tol"], "%s action entropy" % kind)
+        torch.autograd.backward((logp, ent), (dev["adv"], dev["old"]))
+        g64, h64 = d["adv"].double(), d["old"].double()
+        onehot = torch.zeros_like(e["p"])
+        onehot[torch.arange(n), d["actions"].clamp(0, a - 1)] = 1.0
+        want = g64[:, None] * (onehot - e["p"]) - h64[:, None] * e["p"] * (e["lp"] + e["h"][:, None])
+        want = torch.where(e["live"][:, None] & e["ok"], want, torch.zeros_like(want))
+        tol = 2 * e["logp_tol"][:, None] * ((g64.abs()[:, None] + h64.abs()[:, None] * (e["lp"].abs() + e["h"][:, None] + 2)) * e["p"]) + 4 * U * g64.abs()[:, None] * onehot
+        half = torch.finfo(dtype).eps / 2
+        close(z.grad, want, tol * (1 + half) + half * want.abs() + torch.finfo(dtype).smallest_normal * half * 2, "%s action_logp grad" % kind)
 
 
 def test_gradient_against_differences(gpu_device):
