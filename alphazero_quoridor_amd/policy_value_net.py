@@ -534,14 +534,30 @@ class PolicyValueNet:
     on the GPU (the rules engine has no CPU path).
     """
 
-    def __init__(self, model_file=None, use_gpu=True, bn_mode="per_leaf", device=None):
+    def __init__(self, model_file=None, use_gpu=True, bn_mode="per_leaf", device=None, optimizer="adam"):
+        """optimizer: "adam" (the reference's), or "muon": orthogonalised updates (optim.Muon, scaled to the size of Adam's, so that
+        one learning rate serves both) for the convolutions and the value head's first layer, Adam for the output layers, biases and
+        norms."""
         self.use_gpu = use_gpu
         self.l2_const = 1e-4
         if device is None:
             device = "cuda:0" if use_gpu else "cpu"
         self.device = torch.device(device)
         self.policy_value_net = policy_value_net(BasicBlock, IN_PLANES, WIDTH).to(self.device)
-        self.optimizer = torch.optim.Adam(self.policy_value_net.parameters(), weight_decay=self.l2_const)
+        if optimizer == "adam":
+            self.optimizer = torch.optim.Adam(self.policy_value_net.parameters(), weight_decay=self.l2_const)
+        elif optimizer == "muon":
+            from . import optim
+
+            if self.device.type != "cuda":
+                raise ValueError("optimizer='muon' needs the network on a GPU")
+            hidden, rest = [], []
+            for name, p in self.policy_value_net.named_parameters():
+                (hidden if p.dim() == 4 or name == "fc1.weight" else rest).append(p)
+            self.optimizer = optim.Chained(optim.Muon(hidden, weight_decay=self.l2_const, adjust_lr="match_rms_adamw"),
+                                           torch.optim.Adam(rest, weight_decay=self.l2_const))
+        else:
+            raise ValueError("optimizer = %r is neither 'adam' nor 'muon'" % (optimizer,))
         self.bn_mode = bn_mode
         if model_file:
             path = model_file if os.path.exists(str(model_file)) else "ckpt/%s.pth" % model_file
@@ -602,6 +618,25 @@ class PolicyValueNet:
             entropy = -torch.mean(torch.sum(torch.exp(logp) * logp, 1))
         self.weights_changed()
         return loss.detach(), entropy
+
+    def policy_step_t(self, states, actions, advantages, old_logp, winners, lr, legal=None, ref_logits=None, weights=None, clip=0.2, kl_coef=0.0,
+                      entropy_coef=0.0):
+        """One optimiser step of the clipped policy loss (losses.clipped_policy_loss over the legal moves) plus mse(v, z), on device
+        tensors: states [B,26,9,9], actions int64 [B], advantages / old_logp / winners float32 [B], legal as rules.movegen gives it.
+        Returns (loss, mean entropy) as 0-dim device tensors, like train_step_t, whose gradient averaging over ranks it shares."""
+        from . import losses
+
+        self.optimizer.zero_grad(set_to_none=False)
+        set_learning_rate(self.optimizer, lr)
+        logp, v = self.policy_value_net(states)
+        out = losses.clipped_policy_loss(logp, actions, advantages, old_logp, legal=legal, weights=weights, ref_logits=ref_logits, clip=clip, kl_coef=kl_coef,
+                                         entropy_coef=entropy_coef)
+        loss = F.mse_loss(v.view(-1), winners) + out.loss
+        loss.backward()
+        self._allreduce_grads()
+        self.optimizer.step()
+        self.weights_changed()
+        return loss.detach(), out.entropy.mean()
 
     def _world(self):
         import torch.distributed as dist

@@ -8,7 +8,9 @@ What the reference does one game at a time on the host, this pipeline keeps on t
   ``ReplayBuffer`` (588 B per ply; the reference's deque holds 72 KB of float64 per ply).
 * ``policy_update``: the minibatch is gathered and re-encoded on the device, old/new policies,
   KL, explained variance are device tensors; per epoch ONE scalar crosses to the host (the KL
-  that decides whether to stop early, train.py:79-80).
+  that decides whether to stop early, train.py:79-80).  ``objective="clipped"`` trains on moves drawn
+  from the search's distributions under the clipped policy loss instead, ``optimizer="muon"`` with
+  orthogonalised updates.
 * multi-GPU (one process per GPU, torch.distributed / RCCL): every rank plays its own boards,
   finished tuples are all-gathered into every rank's buffer, all ranks start from rank 0's
   weights and average their gradients, so the replicas stay one model; rank 0 alone writes
@@ -24,6 +26,7 @@ import numpy as np
 import torch
 
 from . import dist as qdist
+from . import losses, rules
 from .engine import REFERENCE_MAX_DEPTH, BoardGroups
 from .mcts import MCTSPlayer
 from .policy_value_net import PolicyValueNet
@@ -33,7 +36,17 @@ from .replay import ReplayBuffer, ShardWriter
 
 class TrainPipeline(object):
     def __init__(self, init_model=None, n_boards=1024, device=None, seed=0, bn_mode="per_leaf",
-                 nn_dtype=torch.float32, use_graph=False, n_groups=1, shard_dir=None, max_depth=REFERENCE_MAX_DEPTH):
+                 nn_dtype=torch.float32, use_graph=False, n_groups=1, shard_dir=None, max_depth=REFERENCE_MAX_DEPTH,
+                 objective="mcts", optimizer="adam"):
+        """objective: what policy_update trains the policy on -- "mcts", the search's visit distributions (the reference's cross entropy),
+        or "clipped", moves drawn from them under the clipped policy loss (losses.clipped_policy_loss) with the KL to the policy before
+        the update.  optimizer: see PolicyValueNet."""
+        if objective not in ("mcts", "clipped"):
+            raise ValueError("objective = %r is neither 'mcts' nor 'clipped'" % (objective,))
+        self.objective = objective
+        self.clip = 0.2               # objective "clipped": the ratio's range, and the weights of KL and entropy
+        self.kl_coef = 0.02
+        self.entropy_coef = 0.01
         self.game = Quoridor()
         # the reference's hyper-parameters, same names and values (train.py:17-31)
         self.learn_rate = 2e-3
@@ -51,7 +64,7 @@ class TrainPipeline(object):
         self.best_win_ratio = 0.0
         self.pure_mcts_playout_num = 1000
         self.pure_mcts_rollout_limit = 1000   # pure_mcts.py:81 `limit`
-        self.policy_value_net = PolicyValueNet(model_file=init_model, bn_mode=bn_mode, device=device)
+        self.policy_value_net = PolicyValueNet(model_file=init_model, bn_mode=bn_mode, device=device, optimizer=optimizer)
         self.data_buffer = ReplayBuffer(self.buffer_size, self.policy_value_net.device)
         self._mcts_player = None
         # engine knobs (new)
@@ -188,15 +201,29 @@ class TrainPipeline(object):
         more than 4 kl_targ away from where it started; afterwards the learning-rate multiplier is
         lowered (KL > 2 kl_targ) or raised (KL < kl_targ / 2) by 1.5 within [0.1, 10]."""
         net = self.policy_value_net
-        states, pi, z = self.data_buffer.sample(self.batch_size)  # random.sample positions, states re-encoded on the GPU
+        if self.objective == "mcts":
+            states, pi, z = self.data_buffer.sample(self.batch_size)  # random.sample positions, states re-encoded on the GPU
+        else:
+            boards, pi, z = self.data_buffer.gather(self.data_buffer.sample_indices(self.batch_size))
+            states, legal = rules.encode(boards), rules.movegen(boards)
         old_probs, old_v = net.policy_value_t(states)
         old_logp = torch.log(old_probs + 1e-10)
+        if self.objective == "clipped":
+            # a move of the search's distribution, its log-probability among the legal ones before the update, and how much better the
+            # game ended than the net had expected
+            moves = torch.multinomial(pi, 1).view(-1)
+            move_logp, advantages = losses.action_logp(old_logp, moves, legal=legal), z - old_v.view(-1)
         loss = entropy = None
         new_v = old_v
         kl = 0.0
         steps = 0
         for _ in range(self.epochs):
-            loss, entropy = net.train_step_t(states, pi, z, self.learn_rate * self.lr_multiplier)
+            lr = self.learn_rate * self.lr_multiplier
+            if self.objective == "mcts":
+                loss, entropy = net.train_step_t(states, pi, z, lr)
+            else:
+                loss, entropy = net.policy_step_t(states, moves, advantages, move_logp, z, lr, legal=legal, ref_logits=old_logp, clip=self.clip,
+                                                  kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
             new_probs, new_v = net.policy_value_t(states)
             kl_t = torch.mean(torch.sum(old_probs * (old_logp - torch.log(new_probs + 1e-10)), dim=1))
             kl = float(self._mean_over_ranks(kl_t))  # the one host read per epoch; identical on all ranks
