@@ -164,9 +164,9 @@ class qz_muon_opts(C.Structure):
 
 def build(force: bool = False) -> str:
     """Compile libqzero_hip.so for gfx950 with hipcc (cross-compiles without a GPU)."""
-    srcs = [os.path.join(CSRC, f) for f in ("qz_kernels.hip", "qz_abi.hip", "qz_nn.hip", "qz_conv.hip", "qz_policy.hip", "qz_ortho.hip", "qz_rules.h", "qz_movegen_pool.h",
+    srcs = [os.path.join(CSRC, f) for f in ("qz_kernels.hip", "qz_abi.hip", "qz_nn.hip", "qz_conv.hip", "qz_policy.hip", "qz_ortho.hip", "qz_autograd.cpp", "qz_rules.h", "qz_movegen_pool.h",
                                            "qz_path_rows.h", "qz_rows.h", "qz_device.h", "qz_policy.h", "qz_ortho.h")] + [HEADER]
-    stale = force or not os.path.exists(LIB_PATH) or any(os.path.getmtime(s) > os.path.getmtime(LIB_PATH) for s in srcs)
+    stale = force or not os.path.exists(LIB_PATH) or not os.path.exists(os.path.join(_HERE, "_autograd.so")) or any(os.path.getmtime(s) > os.path.getmtime(LIB_PATH) for s in srcs)
     if stale:
         subprocess.check_call(["make", "-C", CSRC, "-s"])
     return LIB_PATH

@@ -186,18 +186,20 @@ struct RowOut {
     float logp, loss;  // loss without its KL over logits
     Coef g;
 };
+// (e^x - 1 - x) / x^2 for |x| < 1/2, from the series to x^5 / 7!: what is left out is below 2^-6 / 8! of 0.4 or more, 1e-6, at the
+// edge and falls with x^6.  In KL's terms the series goes that far, and not only to where p - q - q x cancels: p and q each carry
+// the error of their own lse, x that of the difference, and q (e^x - 1 - x) is consistent in itself, so that a common error of x only
+// counts squared.
+__device__ __forceinline__ float series2(float x) {
+    float r = 1.f / 5040.f;
+    r = r * x + 1.f / 720.f;
+    r = r * x + 1.f / 120.f;
+    r = r * x + 1.f / 24.f;
+    r = r * x + 1.f / 6.f;
+    return r * x + 0.5f;
+}
 __device__ __forceinline__ float expm1_minus_x(float x) {  // e^x - 1 - x >= 0
-    if (fabsf(x) < 0.5f) {
-        float r = 1.f / 40320.f;
-        r = r * x + 1.f / 5040.f;
-        r = r * x + 1.f / 720.f;
-        r = r * x + 1.f / 120.f;
-        r = r * x + 1.f / 24.f;
-        r = r * x + 1.f / 6.f;
-        r = r * x + 0.5f;
-        return r * x * x;
-    }
-    return expf(x) - 1.f - x;
+    return fabsf(x) < 0.5f ? series2(x) * x * x : expf(x) - 1.f - x;
 }
 __device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, int64_t act, float za, const Stat& st, const Stat& sq, float scale) {
     RowOut o;
@@ -242,17 +244,7 @@ __device__ __forceinline__ float column(const Coef& g, bool has_q, float z, floa
     if (has_q) {
         const float dq = zq - g.mq, lq = dq - g.lsq, q = exp2_fast(lq * LOG2E);
         const float x = (dz - dq) - (g.ls - g.lsq);
-        float f;
-        if (fabsf(x) < 0.25f) {  // p and q agree to within 25 %: their difference from the series, not from p - q
-            float r = 1.f / 720.f;
-            r = r * x + 1.f / 120.f;
-            r = r * x + 1.f / 24.f;
-            r = r * x + 1.f / 6.f;
-            r = r * x + 0.5f;
-            f = q * (r * x * x);
-        } else {
-            f = q == 0.f ? p : (p - q) - q * x;
-        }
+        const float f = fabsf(x) < 0.5f ? q * (series2(x) * x * x) : q == 0.f ? p : (p - q) - q * x;
         kl += f;
         d += g.beta * (p - q);
     }
@@ -760,21 +752,16 @@ __device__ __forceinline__ void block_sum3(float& a, float& b, float& c, float* 
 // One column without branches, for rows whose coefficients are finite: the same values as column().  -inf in both inputs (an illegal
 // column) gives 0 and no term of KL; x is held below 1e30 so that q = 0 gives the term p and not 0 inf.
 struct FastCoef {
-    float m, ls, mq, lsq, c, eta, eh, beta, shift;  // eh = eta h - c, shift = ls - lsq
+    float m, ls, mq, lsqb, c, eta, eh, beta, shift;  // lsqb = lsq log2 e, eh = eta h - c, shift = ls - lsq
 };
 template <bool HAS_Q>
 __device__ __forceinline__ float column_fast(const FastCoef& g, float z, float zq, float& kl) {
     const float dz = z - g.m, lp = dz - g.ls, p = exp2_fast(lp * LOG2E);
     float d = p * (g.eta * fmaxf(lp, -1e30f) + g.eh);
     if (HAS_Q) {
-        const float dq = zq - g.mq, q = exp2_fast((dq - g.lsq) * LOG2E), x = fminf((dz - dq) - g.shift, 1e30f), pq = p - q;
-        float r = 1.f / 720.f;
-        r = r * x + 1.f / 120.f;
-        r = r * x + 1.f / 24.f;
-        r = r * x + 1.f / 6.f;
-        r = r * x + 0.5f;
-        const float qx = q * x, near = qx * (x * r), far = pq - qx;
-        kl += fabsf(x) < 0.25f ? near : far;
+        const float dq = zq - g.mq, q = exp2_fast(dq * LOG2E - g.lsqb), x = fminf((dz - dq) - g.shift, 1e30f), pq = p - q;
+        const float qx = q * x, near = qx * (x * series2(x)), far = pq - qx;
+        kl += fabsf(x) < 0.5f ? near : far;
         d += g.beta * pq;
     }
     return d;
@@ -871,7 +858,7 @@ __global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P,
         forget(q);
         o = row_terms(P, row, act, za, Stat{m, s, t * LN2}, HAS_Q ? Stat{mq, sq, 0.f} : Stat{0.f, 1.f, 0.f}, scale);
         h = o.g.h;
-        const FastCoef g = {o.g.m, o.g.ls, o.g.mq, o.g.lsq, o.g.c, o.g.eta, o.g.eta * h - o.g.c, o.g.beta, o.g.ls - o.g.lsq};
+        const FastCoef g = {o.g.m, o.g.ls, o.g.mq, o.g.lsq * LOG2E, o.g.c, o.g.eta, o.g.eta * h - o.g.c, o.g.beta, o.g.ls - o.g.lsq};
         if (!finite(g.eh) || !finite(g.eta) || !finite(g.c) || !finite(g.beta) || !finite(g.shift) || !finite(g.m)) {
             kl = row_gradient_slow<T, NT>(R, P, O, row, o.g);
         } else if (O.grad || HAS_Q) {

@@ -1,5 +1,6 @@
 """Policy losses on the GPU: log-probabilities of actions under a legal-move mask, and the clipped policy loss with its KL and
-entropy terms, each with its gradient (csrc/qz_policy.hip through the C ABI: qz_action_logp, qz_policy_loss).
+entropy terms, each with its gradient (csrc/qz_policy.hip through the C ABI: qz_action_logp, qz_policy_loss; the autograd functions
+over them: csrc/qz_autograd.cpp).
 
 ``logits`` are [..., A]: any number of decisions over A actions (float32, bfloat16 or float16; log-probabilities serve as
 logits too).  ``legal`` is None, a mask of bytes or bools [..., A], or packed 32-bit words [..., ceil(A / 32)] -- what
@@ -10,11 +11,9 @@ and -inf otherwise.  Illegal columns may hold anything, NaN included.
 There is no CPU path: tensors on another device than a GPU raise ``QzError(QZ_E_NO_DEVICE)``."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _cabi
 
@@ -100,13 +99,31 @@ def _legal(t, lead, a, device):
     return _unit_rows(t), kind
 
 
-def _struct(z, actions, legal, kind):
-    return _cabi.qz_policy_rows(z.data_ptr(), z.stride(0), z.shape[0], z.shape[1], DTYPES[z.dtype], actions.data_ptr(),
-                                legal.data_ptr() if kind else 0, legal.stride(0) if kind else 0, kind)
+def _autograd():
+    """The autograd functions (csrc/qz_autograd.cpp, built beside the library)."""
+    global _ext
+    if _ext is None:
+        _cabi.load()
+        try:
+            from . import _autograd as ext
+        except ImportError as e:
+            raise _cabi.QzLibraryError("_autograd.so is missing or does not load (%s). Build it with `make -C %s`." % (e, _cabi.CSRC)) from e
+        _ext = ext
+    return _ext
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else 0
+_ext = None
+
+
+def _checked(call, *args):
+    try:
+        return call(*args)
+    except RuntimeError as e:
+        text = str(e)
+        if text.startswith("libqzero_hip error "):  # the library's own refusal, as everywhere in this package
+            code, _, rest = text[len("libqzero_hip error "):].partition(": ")
+            raise _cabi.QzError(int(code), rest.splitlines()[0]) from None
+        raise
 
 
 class _Launch:
@@ -145,45 +162,6 @@ def _refuse_captured_leaf(logits):
                            "the network that makes them run inside the capture too")
 
 
-class _ActionLogp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, actions, legal, kind, want_entropy):
-        n, a = z.shape
-        z = _unit_rows(z)
-        need = ctx.needs_input_grad[0]
-        logp, entropy, stats = _logp(z, actions, legal, kind, want_entropy, need)
-        if need:
-            ctx.kind = kind
-            ctx.save_for_backward(z, actions, legal, stats, entropy)
-            ctx.set_materialize_grads(False)
-        return (logp, entropy) if want_entropy else logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp, dentropy=None):
-        z, actions, legal, stats, entropy = ctx.saved_tensors
-        if dlogp is None and dentropy is None:
-            return None, None, None, None, None
-        dlogp = dlogp.contiguous() if dlogp is not None else None
-        dentropy = dentropy.contiguous() if dentropy is not None else None
-        grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        _call(z.device, _cabi.load().qz_action_logp_backward, _struct(z, actions, legal, ctx.kind), stats.data_ptr(), _ptr(entropy), _ptr(dlogp),
-              _ptr(dentropy), grad.data_ptr(), z.shape[1])
-        return grad, None, None, None, None
-
-
-def _logp(z, actions, legal, kind, want_entropy, want_stats):
-    n, a = z.shape
-    logp = torch.empty(n, dtype=torch.float32, device=z.device)
-    entropy = torch.empty_like(logp) if want_entropy else None
-    stats = torch.empty((2, n), dtype=torch.float32, device=z.device) if want_stats else None
-    L = _cabi.load()
-    size = L.qz_policy_workspace(n, a)
-    ws = torch.empty(size, dtype=torch.uint8, device=z.device) if size else None
-    _call(z.device, L.qz_action_logp, _struct(z, actions, legal, kind), logp.data_ptr(), _ptr(entropy), _ptr(stats), _ptr(ws), size)
-    return logp, entropy, stats
-
-
 def action_logp(logits, actions, legal=None, entropy=False):
     """log pi(action) of every decision, float32 with the shape of ``actions``; with ``entropy=True`` a pair of that and the
     entropy of the distribution over the legal actions.  Differentiable in ``logits``."""
@@ -192,74 +170,10 @@ def action_logp(logits, actions, legal=None, entropy=False):
     _refuse_captured_leaf(logits)
     acts = _actions(actions, lead, z.device)
     mask, kind = _legal(legal, lead, z.shape[1], z.device)
-    if z.requires_grad and torch.is_grad_enabled():
-        out = _ActionLogp.apply(z, acts, mask, kind, bool(entropy))
-        logp, ent = out if entropy else (out, None)
-    else:
-        logp, ent, _ = _logp(_unit_rows(z), acts, mask, kind, bool(entropy), False)
+    logp, ent = _checked(_autograd().action_logp, _unit_rows(z), acts, mask, kind, bool(entropy))
     if len(lead) != 1:
         logp, ent = logp.reshape(lead), ent.reshape(lead) if entropy else None
     return (logp, ent) if entropy else logp
-
-
-class _Terms(NamedTuple):
-    clip_low: float
-    clip_high: float
-    kl_coef: float
-    entropy_coef: float
-    kind: int
-
-    def struct(self, advantages, old_logp, ref_logp, weights, ref):
-        return _cabi.qz_policy_terms(advantages.data_ptr(), old_logp.data_ptr(), _ptr(ref_logp), _ptr(weights), _ptr(ref),
-                                     ref.stride(0) if ref is not None else 0, self.clip_low, self.clip_high, self.kl_coef, self.entropy_coef)
-
-
-def _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, want_grad):
-    """-> loss, logp, kl, entropy, gradient or None, and the call's two structs and its workspace (the backward pass's too)."""
-    n, a = z.shape
-    L = _cabi.load()
-    size = L.qz_policy_workspace(n, a)
-    head = (size + 15) & ~15
-    # one allocation: workspace | logp | kl | entropy | loss
-    buf = torch.empty(head + 12 * n + 4, dtype=torch.uint8, device=z.device)
-    logp, kl, entropy, loss = buf[head:].view(torch.float32).split([n, n, n, 1])
-    loss = loss.view(())
-    grad = torch.empty((n, a), dtype=z.dtype, device=z.device) if want_grad else None
-    rows, t = _struct(z, actions, legal, terms.kind), terms.struct(advantages, old_logp, ref_logp, weights, ref)
-    at = buf.data_ptr()
-    out = at + head
-    _call(z.device, L.qz_policy_loss, rows, t, out + 12 * n, out, out + 4 * n, out + 8 * n, _ptr(grad), a, at, size)
-    return loss, logp, kl, entropy, grad, (rows, t, buf, size)
-
-
-class _ClippedPolicyLoss(torch.autograd.Function):
-    """The forward pass writes the gradient for an upstream factor of 1 beside the loss (one pass over the logits for both);
-    the backward pass hands it out, or computes it again where the factor is another or it was handed out before."""
-
-    @staticmethod
-    def forward(ctx, z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms):
-        z = _unit_rows(z)
-        loss, logp, kl, entropy, ctx.grad, ctx.call = _run_loss(z, actions, legal, advantages, old_logp, ref_logp, weights, ref, terms, True)
-        ctx.save_for_backward(z, actions, legal, advantages, old_logp, ref_logp, weights, ref)
-        ctx.mark_non_differentiable(logp, kl, entropy)
-        ctx.set_materialize_grads(False)
-        return loss, logp, kl, entropy
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, upstream, *_):
-        z = ctx.saved_tensors[0]  # (checks that none of them was changed in place; the structs hold their addresses)
-        if upstream is None:
-            return (None,) * 9
-        rows, t, ws, size = ctx.call
-        grad, ctx.grad = ctx.grad, None
-        kept = grad is not None
-        if not kept:  # a second backward pass: computed again, with a workspace of its own
-            grad = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-            ws = torch.empty(max(size, 1), dtype=torch.uint8, device=z.device)
-        upstream = upstream.contiguous()
-        _call(z.device, _cabi.load().qz_policy_loss_backward, rows, t, upstream.data_ptr(), kept, grad.data_ptr(), z.shape[1], ws.data_ptr(), size)
-        return grad, None, None, None, None, None, None, None, None
 
 
 def _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef):
@@ -282,9 +196,9 @@ def _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_l
     if advantages is None or old_logp is None:
         raise TypeError("advantages and old_logp are needed")
     mask, kind = _legal(legal, lead, z.shape[1], device)
-    terms = _Terms(low, high, float(kl_coef), float(entropy_coef), kind)
-    return (z, _actions(actions, lead, device), mask, _vector(advantages, lead, device, "advantages"), _vector(old_logp, lead, device, "old_logp"),
-            _vector(ref_logp, lead, device, "ref_logp"), _vector(weights, lead, device, "weights"), ref, terms), lead
+    return (_unit_rows(z), _actions(actions, lead, device), mask, kind, _vector(advantages, lead, device, "advantages"),
+            _vector(old_logp, lead, device, "old_logp"), _vector(ref_logp, lead, device, "ref_logp"), _vector(weights, lead, device, "weights"), ref, low, high,
+            float(kl_coef), float(entropy_coef)), lead
 
 
 def clipped_policy_loss(logits, actions, advantages, old_logp, legal: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
@@ -298,10 +212,7 @@ def clipped_policy_loss(logits, actions, advantages, old_logp, legal: Optional[t
     Differentiable in ``logits``; memory for their gradient is taken in the forward pass."""
     args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
     _refuse_captured_leaf(logits)
-    if args[0].requires_grad and torch.is_grad_enabled():
-        loss, logp, kl, entropy = _ClippedPolicyLoss.apply(*args)
-    else:
-        loss, logp, kl, entropy, _, _ = _run_loss(_unit_rows(args[0]), *args[1:], False)
+    loss, logp, kl, entropy, _ = _checked(_autograd().policy_loss, *args, False)
     return _result(loss, logp, kl, entropy, lead)
 
 
@@ -316,6 +227,5 @@ def policy_loss_and_grad(logits, actions, advantages, old_logp, legal=None, weig
                          entropy_coef=0.0):
     """(PolicyLoss, gradient of its loss in the logits) without the autograd graph: what a captured HIP graph records."""
     args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
-    z = _unit_rows(args[0])
-    loss, logp, kl, entropy, grad, _ = _run_loss(z, *args[1:], True)
+    loss, logp, kl, entropy, grad = _checked(_autograd().policy_loss, *args, True)
     return _result(loss, logp, kl, entropy, lead), grad.reshape(logits.shape)

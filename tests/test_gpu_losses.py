@@ -395,6 +395,23 @@ def test_upstream_factors_and_a_second_backward(gpu_device, n, a):
         out.loss.backward()
 
 
+def test_no_second_derivative(gpu_device):
+    """create_graph would make autograd take the gradient for a constant: refused."""
+    from alphazero_quoridor_amd import losses
+
+    d = {k: v.to(gpu_device) for k, v in make(4, 12, torch.float32, 1).items()}
+    z = d["z"].requires_grad_(True)
+    for loss in (lambda: losses.clipped_policy_loss(z, d["actions"], d["adv"], d["old"]).loss, lambda: losses.action_logp(z, d["actions"]).sum()):
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(loss(), z, create_graph=True)
+        torch.autograd.grad(loss(), z)
+        out = loss()
+        out.backward()
+        with pytest.raises(RuntimeError, match="second time"):  # the graph was given up
+            out.backward()
+        z.grad = None
+
+
 def test_two_calls_on_two_streams_and_a_captured_call(gpu_device):
     from alphazero_quoridor_amd import losses
 
