@@ -991,9 +991,11 @@ void run_symmetric(Mats& M, int tiles, float* partial, int odd, int last, hipStr
 template <int NP, int KIND>
 void run_gemm(Mats& M, bool may128, float* partial, int odd, int last, hipStream_t s) {
     int tiles = may128 ? set_starts<KIND>(M, 128, 0) : 0;
-    // Tiles of 128 read half as much through LDS per product, tiles of 64 give four times the workgroups: the larger ones unless
-    // there would be next to none.
-    if (tiles < 32) {
+    // Tiles of 128 read half as much through LDS per product, tiles of 64 give four times the workgroups.  B = b A + c A A, whose sum is
+    // short, takes the larger ones where there is one for every other CU (two 1024 x 1024 products, 72 tiles: 15 us in tiles of 64, 23 us
+    // in tiles of 128; six, 216 tiles: 52 us and 45 us); the others, unless there would be next to none (A of two 1024 x 4096: 35 us in
+    // tiles of 64, 33 us in tiles of 128 split along the sum).
+    if (tiles < (KIND == KIND_POLY ? 128 : 32)) {
         tiles = set_starts<KIND>(M, 64, 0);
         if (KIND == KIND_APPLY) hipLaunchKernelGGL((k_ns_gemm<64, NP, KIND, 4>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
         else run_symmetric<NP, KIND, 64>(M, tiles, partial, odd, last, s);
