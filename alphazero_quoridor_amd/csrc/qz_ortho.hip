@@ -256,6 +256,78 @@ __device__ __forceinline__ void store_symmetric(const Mat& m, bool mirror, int r
     }
 }
 
+// A wave's 32 x 64 part of C (rows rb .., columns cb ..; two accumulators side by side) as planes of c_new C + c_old old: to
+// across[column][row], and to along[row][column] too unless the tile lies on the diagonal of a symmetric product.  Through 8 KB of LDS
+// that the stages have left: float32 sums in, rows out (the old values, laid out like `along`, in on the way), then the halves in once
+// more and columns out.  Every access to memory is 16 bytes a lane and 64 bytes or more a row; straight from the accumulators it is 2
+// bytes a lane for rows and 8 bytes a column (1024 x 4096 and its transpose: 56 us a product, 39 us so).
+template <bool OLD>
+__device__ __forceinline__ void store_both(const floatx16 (&acc)[2], char* mine, int rb, int cb, const _Float16* old, _Float16* along, _Float16* across,
+                                           int64_t plane, int64_t ld_along, int64_t ld_across, float c_old, float c_new, bool both) {
+    auto order = [] {  // a wave's LDS accesses keep their order; the compiler is kept to it
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    };
+    const int lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+    float* const f = reinterpret_cast<float*>(mine);         // [32 rows][64 columns]
+    _Float16* const hh = reinterpret_cast<_Float16*>(mine);  // [hi | lo][32][64], chunk q of row r at q ^ 2 (r >> 3)
+    half8 hi[4], lo[4];
+    if (OLD) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int id = lane + 64 * i;
+            const int64_t t = (int64_t)(rb + (id >> 3)) * ld_along + cb + 8 * (id & 7);
+            hi[i] = *reinterpret_cast<const half8*>(old + t);
+            lo[i] = *reinterpret_cast<const half8*>(old + plane + t);
+        }
+    }
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) f[(8 * (e >> 2) + 4 * h + (e & 3)) * 64 + 32 * y + r32] = acc[y][e];
+    order();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int id = lane + 64 * i;
+        const int64_t t = (int64_t)(rb + (id >> 3)) * ld_along + cb + 8 * (id & 7);
+        const float4 a = *reinterpret_cast<const float4*>(f + id * 8), b = *reinterpret_cast<const float4*>(f + id * 8 + 4);
+        const float c[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            _Float16 u, w;
+            split(c[e] * c_new + (OLD ? c_old * (((float)hi[i][e] + (float)lo[i][e]) * INV_SCALE) : 0.f), u, w);
+            hi[i][e] = u;
+            lo[i][e] = w;
+        }
+        if (both) {
+            *reinterpret_cast<half8*>(along + t) = hi[i];
+            *reinterpret_cast<half8*>(along + plane + t) = lo[i];
+        }
+    }
+    order();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int id = lane + 64 * i, r = id >> 3, at = r * 64 + (((id & 7) ^ ((r >> 3) << 1)) << 3);
+        *reinterpret_cast<half8*>(hh + at) = hi[i];
+        *reinterpret_cast<half8*>(hh + 2048 + at) = lo[i];
+    }
+    order();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int c = (lane >> 2) + 16 * i, q = lane & 3, at = q * 512 + (((c >> 3) ^ (q << 1)) << 3) + (c & 7);
+        half8 u, w;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            u[e] = hh[at + 64 * e];
+            w[e] = hh[2048 + at + 64 * e];
+        }
+        const int64_t t = (int64_t)(cb + c) * ld_across + rb + 8 * q;
+        *reinterpret_cast<half8*>(across + t) = u;
+        *reinterpret_cast<half8*>(across + plane + t) = w;
+    }
+    order();
+}
+
 // D: stages of K in flight from memory to registers (the LDS holds two): a workgroup of 64-tiles has little arithmetic per stage to
 // cover a load's latency with.
 template <int T, int NP, int KIND, int D>
@@ -358,6 +430,7 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
+            __builtin_amdgcn_s_setprio(1);  // the wave that multiplies goes first: 3 % of a 4096 x 4096 product
 #pragma unroll
             for (int pr = NP == 3 ? 0 : 2; pr < 3; pr++)  // lo hi, hi lo, hi hi; the same accumulator again only after W W others
 #pragma unroll
@@ -365,6 +438,7 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
 #pragma unroll
                     for (int y = 0; y < W; y++)
                         acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][pr == 0 ? NPL - 1 : 0][x], fq[kk][pr == 1 ? NPL - 1 : 0][y], acc[x][y], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             if (kk == 0) place(st ^ 1, rp[(d + 1) % D], rq[(d + 1) % D]);
             __builtin_amdgcn_sched_barrier(0);
@@ -381,6 +455,19 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
 #pragma unroll
                 for (int g = 0; g < 4; g++)
                     dst[((x * W + y) * 4 + g) * 256] = make_float4(acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2], acc[x][y][4 * g + 3]);
+        return;
+    }
+    if constexpr (T == 128) if (KIND != KIND_APPLY || !last) {
+        constexpr bool SYM = KIND != KIND_APPLY;
+        const int64_t plane = (int64_t)m.sp * (SYM ? m.sp : m.lp);
+        const _Float16* old = KIND == KIND_GRAM ? nullptr : KIND == KIND_POLY ? m.a : odd ? m.xt1 : m.xt0;
+        _Float16* along = KIND == KIND_GRAM ? m.a : KIND == KIND_POLY ? m.b : odd ? m.xt0 : m.xt1;
+        _Float16* across = SYM ? along : m.x;
+        const float c_old = KIND == KIND_POLY ? NS_B : NS_A, c_new = KIND == KIND_POLY ? NS_C * INV_SCALE2 : INV_SCALE2;
+#pragma unroll
+        for (int x = 0; x < W; x++)
+            store_both<KIND != KIND_GRAM>(acc[x], reinterpret_cast<char*>(&sm) + wave * 8192, ti * T + wm + 32 * x, tj * T + wn, old, along, across, plane, m.sp,
+                                          SYM ? m.sp : m.lp, c_old, c_new, !SYM || ti != tj);
         return;
     }
     // lane holds C[row0 + 8 (e >> 2) + (e & 3)][col]: four consecutive rows at a time

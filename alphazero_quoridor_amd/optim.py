@@ -71,8 +71,9 @@ class Muon(torch.optim.Optimizer):
 
     Parameters are float32 matrices or convolution weights ([out, ...] counts as [out, the rest]) on one GPU; gradients float32,
     bfloat16 or float16.  ``adjust_lr``: "original" scales a matrix by sqrt(max(1, rows / cols)), "match_rms_adamw" by
-    0.2 sqrt(max(rows, cols)), which gives updates the size of Adam's.  ``lr`` may be a one-element float32 tensor on the GPU:
-    a captured step follows it."""
+    0.2 sqrt(max(rows, cols)), which gives updates the size of Adam's.  A step can be captured into a HIP graph once a first one has
+    made the momentum buffers; ``lr`` may then be a one-element float32 tensor on the GPU, which the replays follow (a number is
+    recorded as it is)."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, ns_steps=5, adjust_lr="original"):
         if not torch.is_tensor(lr) and not lr >= 0.0:
@@ -87,10 +88,15 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("adjust_lr = %r" % (adjust_lr,))
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=bool(nesterov), weight_decay=weight_decay, ns_steps=int(ns_steps),
                                       adjust_lr=adjust_lr))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() < 2 or p.dtype != torch.float32 or not p.is_contiguous():
-                    raise ValueError("Muon takes contiguous float32 matrices, got %s %s" % (tuple(p.shape), p.dtype))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        params = self.param_groups[-1]["params"]
+        for p in params:
+            if p.dim() < 2 or p.dtype != torch.float32 or not p.is_contiguous():
+                raise ValueError("Muon takes contiguous float32 matrices, got %s %s" % (tuple(p.shape), p.dtype))
+        if len({id(p) for p in params}) < len(params):
+            raise ValueError("the same parameter twice")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -110,6 +116,9 @@ class Muon(torch.optim.Optimizer):
                 buf = state.get("momentum_buffer")
                 if buf is None:
                     _gpu(p, "parameter")
+                    if torch.cuda.is_current_stream_capturing():
+                        # (the capture would record the zeroing, and every replay forget the momentum)
+                        raise RuntimeError("the first step makes the momentum buffers: take one step before the capture")
                     buf = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 if buf.shape != p.shape or buf.dtype is not torch.float32 or p.dtype is not torch.float32 or buf.device != p.device \
                         or not buf.is_contiguous() or not p.is_contiguous():
@@ -135,6 +144,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("a learning rate on the GPU must be one float32 on the parameters' device")
         opts = _cabi.qz_muon_opts(0.0 if lr_dev is not None else float(lr), group["momentum"], group["weight_decay"], int(group["nesterov"]),
                                   lr_dev.data_ptr() if lr_dev is not None else 0)
+        if len(set(words[7::9])) < len(words) // 9:
+            raise ValueError("two parameters share their memory: their updates would race")
         lst = _List(words, device)
         _call(device, _cabi.load().qz_muon_step, lst.ptr, lst.count, DTYPES[dtype], group["ns_steps"], opts, lst.ws.data_ptr(), lst.size)
 

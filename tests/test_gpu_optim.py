@@ -256,6 +256,25 @@ def test_captured_step_follows_the_learning_rate(gpu_device):
             assert torch.equal(p, s), k
 
 
+def test_first_step_in_a_capture_and_shared_memory_are_refused(gpu_device):
+    from alphazero_quoridor_amd import optim
+
+    p = torch.nn.Parameter(gradient(64, 64, 1).to(gpu_device))
+    p.grad = gradient(64, 64, 2).to(gpu_device)
+    opt = optim.Muon([p])
+    before = p.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            opt.step()
+    assert torch.equal(p, before)
+    q = torch.nn.Parameter(p.detach())
+    q.grad = p.grad
+    with pytest.raises(ValueError, match="share their memory"):
+        optim.Muon([p, q]).step()
+    assert torch.equal(p, before)
+
+
 def test_two_lists_on_two_streams(gpu_device):
     from alphazero_quoridor_amd import optim
 

@@ -111,6 +111,22 @@ def test_muon_refuses_bad_options():
             optim.Muon([torch.nn.Parameter(bad)])
 
 
+def test_muon_refuses_a_parameter_twice_and_checks_later_groups():
+    from alphazero_quoridor_amd import optim
+
+    p, q = (torch.nn.Parameter(torch.zeros(3, 5)) for _ in range(2))
+    with pytest.raises(ValueError), pytest.warns(UserWarning):
+        optim.Muon([p, p])
+    opt = optim.Muon([p])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [p]})
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))]})
+    opt = optim.Muon([p])
+    opt.add_param_group({"params": [q], "lr": 0.5})
+    assert opt.param_groups[1]["lr"] == 0.5 and opt.param_groups[1]["momentum"] == 0.95
+
+
 def test_chained_optimisers_step_and_keep_their_state():
     from alphazero_quoridor_amd import optim
 
