@@ -53,11 +53,12 @@ struct Mats {
     OrthoStep o;
 };
 // What one launch of the product kernel covers: tiles base .. of its list, whole (quarters = 0) or as four tiles of half the side.
-// kc > 0: every tile's sum is split into pieces of kc stages, whose partial sums go to `partial`, one tile's worth per workgroup.
+// kc > 0: every tile's sum is split into pieces of about kc stages, whose partial sums go to `partial`, one tile's worth per workgroup.
 struct Part {
     int32_t base, quarters, odd, last, kc;
     float* partial;
 };
+__host__ __device__ constexpr int pieces_of(int stages, int kc) { return stages < kc ? 1 : (stages + kc / 2) / kc; }
 static_assert(sizeof(Mats) + 64 <= 4096, "kernel arguments");
 
 __device__ __forceinline__ int find_mat(const Mats& M, int wg) {
@@ -350,10 +351,10 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
     int ks = 0, ke = K / BK;
     const int slot = wg;
     if (part.kc) {
-        const int pieces = (ke + part.kc - 1) / part.kc, piece = wg % pieces;
+        const int pieces = pieces_of(ke, part.kc), piece = wg % pieces, len = (ke + pieces - 1) / pieces;
         wg /= pieces;
-        ks = piece * part.kc;
-        if (ks + part.kc < ke) ke = ks + part.kc;
+        ks = piece * len;
+        if (ks + len < ke) ke = ks + len;
     }
     const int side = part.quarters ? 2 * T : T;
     int ti, tj;  // tile of P rows, of Q rows
@@ -536,7 +537,7 @@ __global__ __launch_bounds__(256) void k_ns_join(Mats M, Part part) {
     const int wg = blockIdx.x - M.start[i], x = blockIdx.y / (4 * W), y = blockIdx.y / 4 % W, g = blockIdx.y % 4;
     int ti, tj;
     tile_lower(wg, m.sp / T, ti, tj);
-    const int stages = (KIND == KIND_GRAM ? m.lp : m.sp) / BK, pieces = (stages + part.kc - 1) / part.kc;
+    const int stages = (KIND == KIND_GRAM ? m.lp : m.sp) / BK, pieces = pieces_of(stages, part.kc);
     const float4* src = reinterpret_cast<const float4*>(part.partial + (int64_t)(m.pbase + wg * pieces) * T * T) + blockIdx.y * 256 + threadIdx.x;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int p = 0; p < pieces; p++) {
@@ -1038,7 +1039,8 @@ int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
 
 // A symmetric product of fewer tiles than this is split along K, into about SPLIT_GOAL workgroups of at least SPLIT_MIN stages: alone
 // on its CU a workgroup of four waves waits for its own LDS reads most of the time, two or three of them fill the gaps.
-constexpr int SPLIT_BELOW = 384, SPLIT_GOAL = 768, SPLIT_MIN = 16;
+// (480 pieces, so that all of them run at once: of 768, a third ran in a second round.)
+constexpr int SPLIT_BELOW = 384, SPLIT_GOAL = 480, SPLIT_MIN = 16;
 constexpr int SLOTS = 512;  // workgroups of 128-tiles that run at once: two on each of 256 CUs
 
 // -> workgroups; M.start (and pbase) set for tiles of T, split into pieces of kc stages if kc > 0
@@ -1048,7 +1050,7 @@ int set_starts(Mats& M, int T, int kc) {
     for (int i = 0; i < M.count; i++) {
         M.start[i] = wgs;
         const int t = M.m[i].sp / T, nk = (KIND == KIND_GRAM ? M.m[i].lp : M.m[i].sp) / BK;
-        wgs += KIND == KIND_APPLY ? t * (M.m[i].lp / T) : t * (t + 1) / 2 * (kc ? (nk + kc - 1) / kc : 1);
+        wgs += KIND == KIND_APPLY ? t * (M.m[i].lp / T) : t * (t + 1) / 2 * (kc ? pieces_of(nk, kc) : 1);
         if (kc) M.m[i].pbase = M.start[i];
     }
     return wgs;

@@ -28,7 +28,7 @@ def gradient(m, n, seed, noise=0.3):
 
 
 def spectral(m):
-    return float(torch.linalg.matrix_norm(m, 2))
+    return float(torch.linalg.eigvalsh(m @ m.t() if m.shape[0] <= m.shape[1] else m.t() @ m).clamp(min=0).max().sqrt())
 
 
 def iterate(u, steps, v):
@@ -64,6 +64,17 @@ SHAPES = ((1, 1), (1, 2), (2, 1), (1, 128), (3, 5), (4, 576), (2, 576), (15, 17)
 @pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16), ids=("f32", "bf16", "f16"))
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%d" % s)
 def test_orthogonalize(gpu_device, shape, dtype):
+    from alphazero_quoridor_amd import optim
+
+    u = gradient(*shape, seed=shape[0] * 7 + shape[1]).to(dtype)
+    check(optim.orthogonalize(u.to(gpu_device)), u)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16), ids=("f32", "bf16"))
+@pytest.mark.parametrize("shape", ((10, 9000), (16, 8192), (16, 8193), (20, 9000), (40, 2048), (40, 2049), (64, 2100), (100, 512), (100, 513), (128, 600), (130, 9000), (9000, 130),
+                                   (600, 5000), (5000, 520), (1, 70001), (1024, 4100)), ids=lambda s: "%dx%d" % s)
+def test_long_sides(gpu_device, shape, dtype):
+    """Both sides of every border between the ways a matrix is worked on, and sums split over workgroups."""
     from alphazero_quoridor_amd import optim
 
     u = gradient(*shape, seed=shape[0] * 7 + shape[1]).to(dtype)
