@@ -186,6 +186,8 @@ __global__ __launch_bounds__(256) void k_ns_split(Mats M) {
 }
 
 // ---- C = P Q^T, one TxT tile per workgroup of four waves (2 x 2), K in steps of 32 through LDS.
+// Measured at 4096^3: the product with X 465 us (885 TFLOP/s of fp16 products; this card's library product reaches 1,163), the matrix
+// pipe busy for half of the cycles at 1.9 GHz, LDS reads and writes about as long; no bank conflicts; L2 hits 88 %.
 // LDS rows are 64 bytes = four 16-byte chunks; chunk q of row r sits at q ^ ((r >> 2) & 3), so that the sixteen lanes that one
 // pass of a 16-byte read serves fall on sixteen different bank groups.
 enum { KIND_GRAM = 0, KIND_POLY = 1, KIND_APPLY = 2 };
@@ -415,8 +417,8 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
         // unconditional (past the end: the last stage once more), so that the loads in flight are the same on every path and the
         // compiler waits for the oldest only
         fetch(rp[d], rq[d], (k + D < ke ? k + D : ke - 1) * BK);
-        // all fragments of the stage are asked for at once, and the next stage is written between the two halves of the products: a
-        // workgroup alone on its CU then waits for one LDS round trip per stage instead of three
+        // all fragments of the stage are asked for at once, and the next stage is written between the two halves of the products (no
+        // faster than half by half with two workgroups on a CU)
         half8 fp[2][NPL][W], fq[2][NPL][W];
 #pragma unroll
         for (int kk = 0; kk < 2; kk++)  // 16 of K each

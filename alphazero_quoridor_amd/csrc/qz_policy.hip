@@ -265,9 +265,11 @@ __device__ __forceinline__ float wave_sum(float v) {
 __device__ __forceinline__ float wave_max(float v) {
     return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
 }
+// of 2 FROM neighbouring lanes
+template <int FROM>
 __device__ __forceinline__ Stat wave_join(Stat s) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
+    for (int o = FROM; o > 0; o >>= 1) {
         Stat b = {__shfl_xor(s.m, o), __shfl_xor(s.s, o), __shfl_xor(s.t, o)};
         // both lanes of a pair join in the same order, so that all lanes end with the same bits
         s = (threadIdx.x & o) ? stat_join(b, s) : stat_join(s, b);
@@ -276,7 +278,8 @@ __device__ __forceinline__ Stat wave_join(Stat s) {
 }
 template <int NT>
 __device__ __forceinline__ Stat block_join(Stat s, float* sh /*[3 * NT / 64]*/) {
-    s = wave_join(s);
+    constexpr int NW = NT / 64;
+    s = wave_join<32>(s);
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
         sh[3 * wave] = s.m;
@@ -284,8 +287,8 @@ __device__ __forceinline__ Stat block_join(Stat s, float* sh /*[3 * NT / 64]*/) 
         sh[3 * wave + 2] = s.t;
     }
     __syncthreads();
-    Stat r = {sh[0], sh[1], sh[2]};
-    for (int w = 1; w < NT / 64; w++) r = stat_join(r, Stat{sh[3 * w], sh[3 * w + 1], sh[3 * w + 2]});
+    const int w = threadIdx.x & (NW - 1);  // every wave joins all of them, a lane each: one after the other took 1 us of sixteen waves
+    const Stat r = wave_join<NW / 2>(Stat{sh[3 * w], sh[3 * w + 1], sh[3 * w + 2]});
     __syncthreads();
     return r;
 }
@@ -370,6 +373,79 @@ __device__ __forceinline__ void stat_chunk(Stat& st, const Raw& raw) {
         st.s += e;
         st.t += e * fmaxf(x, -1e30f);
     }
+}
+
+// ---- a row's gradient
+// One column without branches, for rows whose coefficients are finite: the same values as column().  -inf in both inputs (an illegal
+// column) gives 0 and no term of KL; x is held below 1e30 so that q = 0 gives the term p and not 0 inf.
+struct FastCoef {
+    float m, ls, mq, lsqb, c, eta, eh, beta, shift;  // lsqb = lsq log2 e, eh = eta h - c, shift = ls - lsq
+};
+template <bool HAS_Q>
+__device__ __forceinline__ float column_fast(const FastCoef& g, float z, float zq, float& kl) {
+    const float dz = z - g.m, lp = dz - g.ls, p = exp2_fast(lp * LOG2E);
+    float d = p * (g.eta * fmaxf(lp, -1e30f) + g.eh);
+    if (HAS_Q) {
+        const float dq = zq - g.mq, q = exp2_fast(dq * LOG2E - g.lsqb), x = fminf((dz - dq) - g.shift, 1e30f), pq = p - q;
+        const float qx = q * x, near = qx * (x * series2(x)), far = pq - qx;
+        kl += fabsf(x) < 0.5f ? near : far;
+        d += g.beta * pq;
+    }
+    return d;
+}
+// a row with an infinite or NaN coefficient: its gradient column by column from memory
+template <typename T, int NT>
+__device__ __forceinline__ float row_gradient_slow(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, int64_t row, const Coef& g, int64_t j0 = 0, int64_t j1 = INT64_MAX) {
+    float kl = 0.f;
+    const bool has_q = P.ref_logits != nullptr;
+#pragma unroll 1
+    for (int64_t j = j0 + threadIdx.x; j < (j1 < R.a ? j1 : R.a); j += NT) {
+        float d = 0.f;
+        if (legal_one(R, row, j))
+            d = column(g, has_q, Elem<T>::get(static_cast<const T*>(R.logits) + row * R.ld, j), has_q ? Elem<T>::get(static_cast<const T*>(P.ref_logits) + row * P.ref_ld, j) : 0.f, j, kl);
+        if (O.grad) Elem<T>::put(static_cast<T*>(O.grad) + row * O.ld_grad, j, d);
+    }
+    return kl;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+
+__device__ __forceinline__ FastCoef fast_coef(const Coef& g) { return {g.m, g.ls, g.mq, g.lsq * LOG2E, g.c, g.eta, g.eta * g.h - g.c, g.beta, g.ls - g.lsq}; }
+__device__ __forceinline__ bool all_finite(const FastCoef& g) {
+    return finite(g.eh) && finite(g.eta) && finite(g.c) && finite(g.beta) && finite(g.shift) && finite(g.m);
+}
+
+// Measured: log-probabilities of 4,096 x 32,000 bfloat16 82 us (3.2 TB/s), their backward pass 90 us (5.8 TB/s, part of it from the caches).
+// columns j0 .. j1 of a row from memory, two chunks in flight; -> this thread's part of KL
+template <typename T, int RT, bool HAS_Q>
+__device__ __forceinline__ float row_gradient(const PolicyRows& R, const PolicyOut& O, const FastCoef& g, const T* z, const T* zq, T* out, int64_t row, int act,
+                                              int64_t j0, int64_t j1) {
+    constexpr int V = Elem<T>::V, STEP = RT * V;
+    float kl = 0.f;
+    for (int64_t j = j0 + (int64_t)threadIdx.x * V; j < j1; j += 2 * STEP) {
+        Raw r[2], q[2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            r[c] = q[c] = raw_empty<T>();
+            if (j + c * STEP < j1) {
+                r[c] = load_legal<T>(R, z, row, j + c * STEP);
+                if (HAS_Q) q[c] = load_legal<T>(R, zq, row, j + c * STEP);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int64_t at = j + c * STEP;
+            if (at >= j1) break;
+            float d[V];
+#pragma unroll
+            for (int k = 0; k < V; k++) d[k] = column_fast<HAS_Q>(g, chunk_get<T>(r[c], k), HAS_Q ? chunk_get<T>(q[c], k) : 0.f, kl);
+            if ((uint64_t)(act - at) < (uint64_t)V) {
+#pragma unroll
+                for (int k = 0; k < V; k++) d[k] += act - at == k ? g.c : 0.f;
+            }
+            if (O.grad) store_chunk<T>(out, at, R.a, d);
+        }
+    }
+    return kl;
 }
 
 // ================================================================ any width: one workgroup per row, the row read twice
@@ -457,18 +533,13 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
         o = row_terms(P, row, act, za, st, sq, scale);
         const T* z = static_cast<const T*>(R.logits) + row * R.ld;
         const T* zq = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
-        if (O.grad || has_q) {
-            for (int64_t j = (int64_t)threadIdx.x * V; j < R.a; j += RT * V) {
-                const uint32_t ok = legal_bits<V>(R, row, j);
-                const Raw raw = load_chunk<T>(z, j, R.a);
-                Raw rq = {};
-                if (has_q) rq = load_chunk<T>(zq, j, R.a);
-                float d[V];
-#pragma unroll
-                for (int k = 0; k < V; k++)
-                    d[k] = (ok >> k) & 1u ? column(o.g, has_q, chunk_get<T>(raw, k), has_q ? chunk_get<T>(rq, k) : 0.f, j + k, kl) : 0.f;
-                if (O.grad) store_chunk<T>(out, j, R.a, d);
-            }
+        const FastCoef g = fast_coef(o.g);
+        if (!all_finite(g)) {
+            kl = row_gradient_slow<T, RT>(R, P, O, row, o.g);
+        } else if (has_q) {
+            kl = row_gradient<T, RT, true>(R, O, g, z, zq, out, row, (int)act, 0, R.a);
+        } else if (O.grad) {
+            row_gradient<T, RT, false>(R, O, g, z, zq, out, row, (int)act, 0, R.a);
         }
         kl = has_q ? block_sum<RT>(kl, sh) : kl_taken(P, row, o.logp);
     } else if (O.grad) {
@@ -510,7 +581,7 @@ __global__ __launch_bounds__(ST) void k_split_stats(PolicyRows R, PolicyTerms P,
 __device__ __forceinline__ Stat split_join(const Split& S, int64_t row, int k) {
     const int lane = threadIdx.x & 63;
     const float* in = S.stats + ((row * 2 + k) * S.s + lane) * 3;
-    return wave_join(lane < S.s ? Stat{in[0], in[1], in[2]} : Stat{LOWEST, 0.f, 0.f});
+    return wave_join<32>(lane < S.s ? Stat{in[0], in[1], in[2]} : Stat{LOWEST, 0.f, 0.f});
 }
 template <typename T>
 __global__ __launch_bounds__(64) void k_split_logp(PolicyRows R, Split S, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
@@ -546,19 +617,10 @@ __global__ __launch_bounds__(ST) void k_split_loss(PolicyRows R, PolicyTerms P, 
         o = row_terms(P, row, act, za, split_join(S, row, 0), has_q ? split_join(S, row, 1) : Stat{0.f, 1.f, 0.f}, scale);
         const T* z = static_cast<const T*>(R.logits) + row * R.ld;
         const T* zq = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
-        if (O.grad || has_q) {
-            for (int64_t j = j0 + (int64_t)threadIdx.x * V; j < j1; j += ST * V) {
-                const uint32_t ok = legal_bits<V>(R, row, j);
-                const Raw raw = load_chunk<T>(z, j, R.a);
-                Raw rq = {};
-                if (has_q) rq = load_chunk<T>(zq, j, R.a);
-                float d[V];
-#pragma unroll
-                for (int k = 0; k < V; k++)
-                    d[k] = (ok >> k) & 1u ? column(o.g, has_q, chunk_get<T>(raw, k), has_q ? chunk_get<T>(rq, k) : 0.f, j + k, kl) : 0.f;
-                if (O.grad) store_chunk<T>(out, j, R.a, d);
-            }
-        }
+        const FastCoef g = fast_coef(o.g);
+        if (!all_finite(g)) kl = row_gradient_slow<T, ST>(R, P, O, row, o.g, j0, j1);
+        else if (has_q) kl = row_gradient<T, ST, true>(R, O, g, z, zq, out, row, (int)act, j0, j1);
+        else if (O.grad) row_gradient<T, ST, false>(R, O, g, z, zq, out, row, (int)act, j0, j1);
         if (has_q) kl = block_sum<ST>(kl, sh);
     } else if (O.grad) {
         const float zero[V] = {};
@@ -600,7 +662,7 @@ __global__ __launch_bounds__(256) void k_split_finish(PolicyOut O, Split S, int 
 }
 
 // ================================================================ narrow rows: a wave per row, the row in registers
-// Bound by launch and memory latency at the sizes that boards have (13,312 rows of 140); four rows per workgroup.
+// Bound by launch and memory latency at the sizes that boards have (13,312 rows of 140: 7 us, 1.1 TB/s); four rows per workgroup.
 template <typename T>
 __device__ __forceinline__ float masked(const PolicyRows& R, int64_t row, const void* base, int64_t ld, int64_t j) {
     if (j >= R.a || !legal_one(R, row, j)) return NEG_INF;
@@ -695,6 +757,7 @@ __global__ __launch_bounds__(256) void k_wave_loss(PolicyRows R, PolicyTerms P, 
 }
 
 // ================================================================ wide rows: a workgroup per row, the row in registers
+// (8,192 x 32,768 bfloat16 with a frozen policy's logits, 1.6 GB: 410 us, 3.9 TB/s; a copy reaches 4.6.)
 // One pass over memory: logits (and the frozen policy's) are read once, into registers as they are stored, illegal columns replaced by
 // -inf on the way; then the maximum, the sums and the gradient come from the registers.  Bound by memory where there is one input, by
 // vector instructions (~50 per column with two inputs) close behind it otherwise; two workgroups of 512 share a CU, so that one's
@@ -749,39 +812,6 @@ __device__ __forceinline__ void block_sum3(float& a, float& b, float& c, float* 
         c += sh[32 + w];
     }
 }
-// One column without branches, for rows whose coefficients are finite: the same values as column().  -inf in both inputs (an illegal
-// column) gives 0 and no term of KL; x is held below 1e30 so that q = 0 gives the term p and not 0 inf.
-struct FastCoef {
-    float m, ls, mq, lsqb, c, eta, eh, beta, shift;  // lsqb = lsq log2 e, eh = eta h - c, shift = ls - lsq
-};
-template <bool HAS_Q>
-__device__ __forceinline__ float column_fast(const FastCoef& g, float z, float zq, float& kl) {
-    const float dz = z - g.m, lp = dz - g.ls, p = exp2_fast(lp * LOG2E);
-    float d = p * (g.eta * fmaxf(lp, -1e30f) + g.eh);
-    if (HAS_Q) {
-        const float dq = zq - g.mq, q = exp2_fast(dq * LOG2E - g.lsqb), x = fminf((dz - dq) - g.shift, 1e30f), pq = p - q;
-        const float qx = q * x, near = qx * (x * series2(x)), far = pq - qx;
-        kl += fabsf(x) < 0.5f ? near : far;
-        d += g.beta * pq;
-    }
-    return d;
-}
-// a row with an infinite or NaN coefficient: its gradient column by column from memory
-template <typename T, int NT>
-__device__ __forceinline__ float row_gradient_slow(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, int64_t row, const Coef& g) {
-    float kl = 0.f;
-    const bool has_q = P.ref_logits != nullptr;
-#pragma unroll 1
-    for (int64_t j = threadIdx.x; j < R.a; j += NT) {
-        float d = 0.f;
-        if (legal_one(R, row, j))
-            d = column(g, has_q, Elem<T>::get(static_cast<const T*>(R.logits) + row * R.ld, j), has_q ? Elem<T>::get(static_cast<const T*>(P.ref_logits) + row * P.ref_ld, j) : 0.f, j, kl);
-        if (O.grad) Elem<T>::put(static_cast<T*>(O.grad) + row * O.ld_grad, j, d);
-    }
-    return kl;
-}
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
-
 // A thread holds CH chunks of 16 bytes, and the first few threads one column each of what is left over of the row.
 template <typename T, int NT, int CH, bool HAS_Q, bool MASK>
 __global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P, PolicyOut O) {
@@ -858,8 +888,8 @@ __global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P,
         forget(q);
         o = row_terms(P, row, act, za, Stat{m, s, t * LN2}, HAS_Q ? Stat{mq, sq, 0.f} : Stat{0.f, 1.f, 0.f}, scale);
         h = o.g.h;
-        const FastCoef g = {o.g.m, o.g.ls, o.g.mq, o.g.lsq * LOG2E, o.g.c, o.g.eta, o.g.eta * h - o.g.c, o.g.beta, o.g.ls - o.g.lsq};
-        if (!finite(g.eh) || !finite(g.eta) || !finite(g.c) || !finite(g.beta) || !finite(g.shift) || !finite(g.m)) {
+        const FastCoef g = fast_coef(o.g);
+        if (!all_finite(g)) {
             kl = row_gradient_slow<T, NT>(R, P, O, row, o.g);
         } else if (O.grad || HAS_Q) {
             const int a32 = (int)act;
@@ -923,13 +953,13 @@ __global__ __launch_bounds__(1024) void k_sum_parts(const double* __restrict__ p
     }
 
 namespace {
-// rows of up to 1,024 columns stay with one wave (16 registers of values per lane); 140 columns take 3
-constexpr int WAVE_WIDEST = 1024;
-#define BY_WIDTH(a, ...)                                    \
-    if ((a) <= 64) { constexpr int E = 1; __VA_ARGS__; }           \
-    else if ((a) <= 192) { constexpr int E = 3; __VA_ARGS__; }     \
-    else if ((a) <= 512) { constexpr int E = 8; __VA_ARGS__; }     \
-    else { constexpr int E = 16; __VA_ARGS__; }
+// Narrow rows stay with one wave (140 columns take 3 registers of values per lane): log-probabilities of 8,192 x 1,000 float32 8 us, and
+// 26 us with a workgroup per row; the loss of 32,768 x 512 56 and 85 us, of 8,192 x 1,000 33 and 30 us.
+constexpr int WAVE_WIDEST = 1024, WAVE_WIDEST_LOSS = 512;
+#define BY_WIDTH(a, ...)                                       \
+    if ((a) <= 64) { constexpr int E = 1; __VA_ARGS__; }       \
+    else if ((a) <= 192) { constexpr int E = 3; __VA_ARGS__; } \
+    else { constexpr int E = 8; __VA_ARGS__; }
 
 template <typename T, int NT, int CH>
 void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
@@ -939,7 +969,13 @@ void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hip
     else if (R.legal_kind) hipLaunchKernelGGL((k_row_loss<T, NT, CH, false, true>), grid, block, 0, s, R, P, O);
     else hipLaunchKernelGGL((k_row_loss<T, NT, CH, false, false>), grid, block, 0, s, R, P, O);
 }
-// the smallest workgroup whose registers hold the row; past 1,024 threads of 8 chunks the row is read twice
+// Rows read from memory twice: with one row per CU or fewer, sixteen waves draw more from memory than four (100 x 100,000 bfloat16 with a
+// frozen policy: 51 us, and 82 us with four); with more rows, four on each of several rows (600 x 100,000: 145 us, and 161 us).
+bool few(int64_t n) { return n <= 256; }
+// The smallest workgroup whose registers hold the row: 8,192 x 32,768 bfloat16 with a frozen policy 410 us, 452 us read twice; without
+// one 206 and 250 us; 2,048 x 4,000 23 and 32 us.  Past 512 threads of 8 chunks the row is read twice: a workgroup of 1,024 would have
+// a CU to itself, and nothing to cover its loads with (2,048 x 50,001: 315 us, 226 us read twice) -- but for one input with a mask, whose
+// second reading costs more (2,047 x 50,001 with a byte mask: 180 us, 191 us read twice).
 template <typename T>
 void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
     const int chunks = (R.a + Elem<T>::V - 1) / Elem<T>::V;
@@ -948,16 +984,17 @@ void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hi
     else if (chunks <= 1024) row_loss<T, 256, 4>(R, P, O, s);
     else if (chunks <= 2048) row_loss<T, 512, 4>(R, P, O, s);
     else if (chunks <= 4096) row_loss<T, 512, 8>(R, P, O, s);
-    else if (chunks <= 8192) row_loss<T, 1024, 8>(R, P, O, s);
-    else if (R.n <= 1024) hipLaunchKernelGGL((k_policy_loss<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
+    else if (chunks <= 8192 && R.legal_kind && !P.ref_logits) hipLaunchKernelGGL((k_row_loss<T, 1024, 8, false, true>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
+    else if (few(R.n)) hipLaunchKernelGGL((k_policy_loss<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
     else hipLaunchKernelGGL((k_policy_loss<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, P, O);
 }
 }  // namespace
 
 namespace {
-// Rows are split where a workgroup each would leave most CUs idle and a row is long enough to be worth three launches.
+// Rows are split where a workgroup each would leave most CUs idle and a row is long enough to be worth three launches: 1 x 131,072
+// bfloat16 with a frozen policy 20 us, and 60 us in one workgroup; 32 x 32,768 18 and 19 us; 64 x 32,768 21 and 19 us.
 constexpr int FEW_ROWS = 64, SPLIT_WIDTH = 32768;
-bool few_wide(int64_t n, int a) { return n <= FEW_ROWS && a >= SPLIT_WIDTH; }
+bool few_wide(int64_t n, int a) { return n <= FEW_ROWS && a >= SPLIT_WIDTH && a >= 1024 * n; }
 Split make_split(int64_t n, int a, int v, void* ws) {
     Split S;
     const int unit = ST * v;  // columns that one pass of a workgroup covers
@@ -979,14 +1016,16 @@ int64_t policy_workspace_bytes(int64_t n, int a) { return n * 8 + (few_wide(n, a
 
 hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void* ws, hipStream_t s) {
     if (R.n <= 0) return hipSuccess;
-    if (R.a <= WAVE_WIDEST) {
+    if (R.a > 512 && R.a <= WAVE_WIDEST) {
+        BY_TYPE(R.dtype, hipLaunchKernelGGL((k_wave_logp<T, 16>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats));
+    } else if (R.a <= 512) {
         BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_logp<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats)));
     } else if (few_wide(R.n, R.a)) {
         const PolicyTerms none = {};
         BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws);
                 hipLaunchKernelGGL((k_split_stats<T>), dim3(S.s, (unsigned)R.n), dim3(ST), 0, s, R, none, S, nullptr, 0);
                 hipLaunchKernelGGL((k_split_logp<T>), dim3((unsigned)R.n), dim3(64), 0, s, R, S, logp, entropy, stats));
-    } else if (R.n <= 1024) {  // up to four rows per CU: more waves on each
+    } else if (few(R.n) && R.a >= 65536) {  // (shorter rows: four waves, 1,024 x 8,192 8 us, and 22 us with sixteen)
         BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, logp, entropy, stats));
     } else {
         BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, logp, entropy, stats));
@@ -1004,7 +1043,7 @@ hipError_t action_logp_backward(const PolicyRows& R, const float* stats, const f
 hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, float* loss, void* ws, hipStream_t s) {
     O.parts = loss ? static_cast<double*>(ws) : nullptr;
     if (R.n > 0) {
-        if (R.a <= WAVE_WIDEST) {
+        if (R.a <= WAVE_WIDEST_LOSS) {
             BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_loss<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, P, O)));
         } else if (few_wide(R.n, R.a)) {
             BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws); const dim3 grid(S.s, (unsigned)R.n);
