@@ -9,9 +9,11 @@
 //   X'^T = a X^T + X^T B (B symmetric): rows of X^T against rows of B.  So X is kept in both orientations.
 // float32 accuracy on the fp16 matrix pipe: every value is hi + lo, two fp16 numbers of the value times 4096 (a 22-bit
 // significand; all entries are below 4 in magnitude, so 4096 keeps hi in range and lo out of the subnormals down to 2^-15), and a
-// product is hi hi + hi lo + lo hi with float32 accumulation.  Where the result is rounded to bfloat16 and the shorter side is
-// 256 or more, ONE product (hi hi) is enough: the term a X, which carries the small singular values through the steps, is still
-// taken from hi + lo, and the error of one product is 1.4e-3 of the result, next to the output's own rounding of 1.7e-3.
+// product is hi hi + hi lo + lo hi with float32 accumulation.  Where the result is rounded to bfloat16 and the matrix is large, ONE
+// product (hi hi) is enough: the term a X, which carries the small singular values through the steps, is still taken from
+// hi + lo.  The error of one product falls with the shorter side s and grows with the longer l: measured together with the output's
+// own rounding (1.66e-3 alone) 1.94e-3 at 1,024^2, 2.07e-3 at 1,024 x 4,096, 1.92e-3 at 1,500 x 8,192, 1.82e-3 at 2,048 x 8,192, but
+// 2.3e-3 at 1,024 x 8,192, 2.1e-3 at 512^2 and 2.9e-3 at 512 x 4,096.  So: s >= 1,024 and s s >= 256 l.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -1004,7 +1006,10 @@ int path_of(int64_t rows, int64_t cols) {
 }
 // Matrices whose shorter side is 512 or more are padded so that tiles of 128 may be used.
 int pad_of(int64_t rows, int64_t cols) { return (rows < cols ? rows : cols) >= 512 ? 128 : 64; }
-bool one_product(const OrthoMatrix& q, const OrthoStep& o) { return !o.muon && o.dtype == 1 && (q.rows < q.cols ? q.rows : q.cols) >= 256; }
+bool one_product(const OrthoMatrix& q, const OrthoStep& o) {
+    const int64_t s = q.rows < q.cols ? q.rows : q.cols, l = q.rows < q.cols ? q.cols : q.rows;
+    return !o.muon && o.dtype == 1 && s >= 1024 && s * s >= 256 * l;
+}
 
 int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
     const int64_t s = q.rows < q.cols ? q.rows : q.cols, l = q.rows < q.cols ? q.cols : q.rows;

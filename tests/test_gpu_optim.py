@@ -81,6 +81,20 @@ def test_long_sides(gpu_device, shape, dtype):
     check(optim.orthogonalize(u.to(gpu_device)), u)
 
 
+@pytest.mark.parametrize("shape", ((256, 1024), (320, 2500), (1536, 384), (700, 640), (512, 4096), (1023, 1100), (1024, 8192), (4097, 1024)), ids=lambda s: "%dx%d" % s)
+def test_bfloat16_results_lose_no_more_than_their_rounding(gpu_device, shape):
+    """Where the shorter side is short, or the longer long beside it, a 16-bit result is as near as the three products of float32
+    results bring it.  Tolerance: with x the kernel's value before rounding, |x - want| = e, the stored value is the nearest to x, so
+    |got - want| <= |got - x| + e <= |bf16(want) - x| + e <= |bf16(want) - want| + 2 e, and e is the split operands' bound."""
+    from alphazero_quoridor_amd import optim
+
+    u = gradient(*shape, seed=shape[0] * 7 + shape[1]).bfloat16()
+    want, bound = iterate(u, 5, 2.0 ** -22)
+    bound = float((want.bfloat16().double() - want).norm()) + 2 * bound
+    off = float((optim.orthogonalize(u.to(gpu_device)).double().cpu() - want).norm())
+    assert off <= bound, "%s: off by %.3g, bound %.3g" % (shape, off, bound)
+
+
 def test_orthogonalize_a_list_equals_its_members(gpu_device):
     """More matrices than one launch takes, of all sizes and types, tall and wide, in one call."""
     from alphazero_quoridor_amd import optim
