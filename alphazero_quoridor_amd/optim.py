@@ -144,7 +144,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("a learning rate on the GPU must be one float32 on the parameters' device")
         opts = _cabi.qz_muon_opts(0.0 if lr_dev is not None else float(lr), group["momentum"], group["weight_decay"], int(group["nesterov"]),
                                   lr_dev.data_ptr() if lr_dev is not None else 0)
-        if len(set(words[7::9])) < len(words) // 9:
+        spans = sorted(zip(words[7::9], words[0::9], words[1::9]))
+        if any(at + 4 * rows * cols > above[0] for (at, rows, cols), above in zip(spans, spans[1:])):
             raise ValueError("two parameters share their memory: their updates would race")
         lst = _List(words, device)
         _call(device, _cabi.load().qz_muon_step, lst.ptr, lst.count, DTYPES[dtype], group["ns_steps"], opts, lst.ws.data_ptr(), lst.size)

@@ -300,6 +300,26 @@ def test_first_step_in_a_capture_and_shared_memory_are_refused(gpu_device):
     assert torch.equal(p, before)
 
 
+def test_overlapping_parameters_are_refused(gpu_device):
+    """Two weights that share some of their memory, neither starting where the other does."""
+    from alphazero_quoridor_amd import optim
+
+    whole = gradient(96, 64, 1).to(gpu_device)
+    before = whole.clone()
+    for cuts in (((0, 64), (32, 96)), ((32, 96), (0, 64)), ((0, 96), (40, 50))):
+        ps = [torch.nn.Parameter(whole[a:b]) for a, b in cuts]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(ValueError, match="share their memory"):
+            optim.Muon(ps).step()
+    assert torch.equal(whole, before)
+    ps = [torch.nn.Parameter(whole[a:b]) for a, b in ((48, 96), (0, 48))]  # side by side is fine
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    optim.Muon(ps).step()
+    assert not torch.equal(whole[:48], before[:48]) and not torch.equal(whole[48:], before[48:])
+
+
 def test_two_lists_on_two_streams(gpu_device):
     from alphazero_quoridor_amd import optim
 
