@@ -49,6 +49,8 @@ def _rows_of(logits, name="logits"):
         raise TypeError("%s: %s is not one of float32, bfloat16, float16" % (name, logits.dtype))
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("%s: at least one action is needed, got the shape %s" % (name, tuple(logits.shape)))
+    if logits.shape[-1] > 1 << 30:
+        raise ValueError("%s: %d actions, at most 2^30 are supported" % (name, logits.shape[-1]))
     return logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
 
 

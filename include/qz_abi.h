@@ -492,7 +492,7 @@ typedef struct {
     const void* logits;             /* [dev] n rows of n_actions elements                              */
     int64_t ld;                     /* elements between rows                                           */
     int64_t n;
-    int32_t n_actions;
+    int32_t n_actions;              /* 1 .. 2^30                                                        */
     int32_t dtype;
     const int64_t* actions;         /* [dev][n]                                                        */
     const void* legal;              /* [dev] or NULL                                                   */

@@ -501,3 +501,15 @@ def test_refusals_on_the_device(gpu_device):
                           (dict(clip=float("nan")), ValueError), (dict(advantages=None), TypeError)):
         with pytest.raises(error):
             losses.clipped_policy_loss(**dict(ok, **change))
+
+
+def test_rows_too_long_to_index_are_refused(gpu_device):
+    """More columns than 32 bits count would wrap to another number: refused before anything is read or copied."""
+    from alphazero_quoridor_amd import losses
+
+    a, f = torch.zeros(1, dtype=torch.int64, device=gpu_device), torch.zeros(1, device=gpu_device)
+    for cols in (2 ** 30 + 1, 2 ** 32 + 5):
+        z = torch.zeros((1, 1), device=gpu_device).expand(1, cols)
+        for call in (lambda: losses.action_logp(z, a), lambda: losses.clipped_policy_loss(z, a, f, f), lambda: losses.policy_loss_and_grad(z, a, f, f)):
+            with pytest.raises(ValueError, match="at most 2\\^30"):
+                call()

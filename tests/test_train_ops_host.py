@@ -53,6 +53,14 @@ def test_policy_entry_points_refuse_bad_arguments():
     assert L.qz_policy_workspace(-1, 140) == 0 and L.qz_policy_workspace(4, 0) == 0
 
 
+def test_rows_too_long_to_index_are_refused():
+    L, p = lib(), 1 << 20
+    for a in ((1 << 30) + 1, (1 << 31) - 1):
+        r = rows(n=1, n_actions=a)
+        assert L.qz_policy_loss(C.byref(r), C.byref(terms()), p, p, p, p, p, 140, p, BIG, None) == _cabi.E_INVALID
+        assert L.qz_action_logp(C.byref(r), p, None, None, p, BIG, None) == _cabi.E_INVALID
+
+
 def test_matrix_entry_points_refuse_bad_arguments():
     L, p = lib(), 1 << 20
 
