@@ -1102,7 +1102,7 @@ int qz_memo_flush(qz_engine* e, void* stream) {
 static int policy_rows(const qz_policy_rows* r, PolicyRows* out) {
     if (!r) return fail(QZ_E_INVALID, "null rows");
     if (r->n < 0 || r->n > 0x7fffffffLL) return fail(QZ_E_INVALID, "n = %lld is not in 0 .. 2^31 - 1", (long long)r->n);
-    if (r->n_actions < 1 || r->n_actions > (1 << 30)) return fail(QZ_E_INVALID, "n_actions = %d is not in 1 .. 2^30", r->n_actions);  // (the kernels step past it in 32 bits)
+    if (r->n_actions < 1 || r->n_actions > (1 << 30)) return fail(QZ_E_INVALID, "n_actions = %d is not in 1 .. 2^30", r->n_actions);  // (launches round a row up to whole tiles in 32 bits)
     if (r->dtype < QZ_F32 || r->dtype > QZ_F16) return fail(QZ_E_INVALID, "unknown element type %d", r->dtype);
     if (r->legal_kind < QZ_LEGAL_ALL || r->legal_kind > QZ_LEGAL_BYTES) return fail(QZ_E_INVALID, "unknown legal_kind %d", r->legal_kind);
     if (r->n > 0 && (!r->logits || !r->actions || (r->legal_kind != QZ_LEGAL_ALL && !r->legal))) return fail(QZ_E_INVALID, "null logits, actions or legal set");
