@@ -9,11 +9,8 @@
 //   X'^T = a X^T + X^T B (B symmetric): rows of X^T against rows of B.  So X is kept in both orientations.
 // float32 accuracy on the fp16 matrix pipe: every value is hi + lo, two fp16 numbers of the value times 4096 (a 22-bit
 // significand; all entries are below 4 in magnitude, so 4096 keeps hi in range and lo out of the subnormals down to 2^-15), and a
-// product is hi hi + hi lo + lo hi with float32 accumulation.  Where the result is rounded to bfloat16 and the matrix is large, ONE
-// product (hi hi) is enough: the term a X, which carries the small singular values through the steps, is still taken from
-// hi + lo.  The error of one product falls with the shorter side s and grows with the longer l: measured together with the output's
-// own rounding (1.66e-3 alone) 1.94e-3 at 1,024^2, 2.07e-3 at 1,024 x 4,096, 1.92e-3 at 1,500 x 8,192, 1.82e-3 at 2,048 x 8,192, but
-// 2.3e-3 at 1,024 x 8,192, 2.1e-3 at 512^2 and 2.9e-3 at 512 x 4,096.  So: s >= 1,024 and s s >= 256 l.
+// product is hi hi + hi lo + lo hi with float32 accumulation, whatever the result's type: hi hi alone leaves a bfloat16 result up to
+// 2.9e-3 off float64 (updates of flat or sparse spectra, 1,024 x 4,096) where its own rounding is 1.66e-3.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -195,10 +192,10 @@ __global__ __launch_bounds__(256) void k_ns_split(Mats M) {
 enum { KIND_GRAM = 0, KIND_POLY = 1, KIND_APPLY = 2 };
 constexpr int BK = 32;
 
-template <int T, int NPL>
+template <int T>
 struct GemmShared {
-    half8 p[2][NPL][T * 4];  // [stage][hi | lo][row, chunk]
-    half8 q[2][NPL][T * 4];
+    half8 p[2][2][T * 4];  // [stage][hi | lo][row, chunk]
+    half8 q[2][2][T * 4];
 };
 
 // Workgroup b runs on XCD b mod 8, each with an L2 of its own: consecutive tiles go to the same XCD.
@@ -335,12 +332,11 @@ __device__ __forceinline__ void store_both(const floatx16 (&acc)[2], char* mine,
 
 // D: stages of K in flight from memory to registers (the LDS holds two): a workgroup of 64-tiles has little arithmetic per stage to
 // cover a load's latency with.
-template <int T, int NP, int KIND, int D>
+template <int T, int KIND, int D>
 __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part part) {
-    constexpr int NPL = NP == 3 ? 2 : 1;  // planes read
     constexpr int W = T / 64;             // 32 x 32 tiles per wave and side
     constexpr int LD = T * 4 / 256;       // 16-byte chunks per thread, operand and plane
-    __shared__ GemmShared<T, NPL> sm;
+    __shared__ GemmShared<T> sm;
     const int odd = part.odd, last = part.last;
     int wg = xcd_order(blockIdx.x, gridDim.x), quarter = 0;
     if (part.quarters) {
@@ -377,10 +373,10 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
     const int wm = (wave >> 1) * (T / 2), wn = (wave & 1) * (T / 2);
     const int r32 = lane & 31, h = lane >> 5;
 
-    half8 rp[D][NPL][LD], rq[D][NPL][LD];
-    auto fetch = [&](half8 (&fp)[NPL][LD], half8 (&fq)[NPL][LD], int k0) {
+    half8 rp[D][2][LD], rq[D][2][LD];
+    auto fetch = [&](half8 (&fp)[2][LD], half8 (&fq)[2][LD], int k0) {
 #pragma unroll
-        for (int pl = 0; pl < NPL; pl++)
+        for (int pl = 0; pl < 2; pl++)
 #pragma unroll
             for (int t = 0; t < LD; t++) {
                 const int c = tid + 256 * t, row = c >> 2, q = c & 3;
@@ -388,9 +384,9 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
                 fq[pl][t] = *reinterpret_cast<const half8*>(Q + pl * q_plane + (int64_t)(tj * T + row) * K + k0 + q * 8);
             }
     };
-    auto place = [&](int st, half8 (&fp)[NPL][LD], half8 (&fq)[NPL][LD]) {
+    auto place = [&](int st, half8 (&fp)[2][LD], half8 (&fq)[2][LD]) {
 #pragma unroll
-        for (int pl = 0; pl < NPL; pl++)
+        for (int pl = 0; pl < 2; pl++)
 #pragma unroll
             for (int t = 0; t < LD; t++) {
                 const int c = tid + 256 * t, row = c >> 2, q = c & 3;
@@ -421,11 +417,11 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
         fetch(rp[d], rq[d], (k + D < ke ? k + D : ke - 1) * BK);
         // all fragments of the stage are asked for at once, and the next stage is written between the two halves of the products (no
         // faster than half by half with two workgroups on a CU)
-        half8 fp[2][NPL][W], fq[2][NPL][W];
+        half8 fp[2][2][W], fq[2][2][W];
 #pragma unroll
         for (int kk = 0; kk < 2; kk++)  // 16 of K each
 #pragma unroll
-            for (int pl = 0; pl < NPL; pl++)
+            for (int pl = 0; pl < 2; pl++)
 #pragma unroll
                 for (int x = 0; x < W; x++) {
                     const int rp_ = wm + 32 * x + r32, rq_ = wn + 32 * x + r32, q = 2 * kk + h;
@@ -437,12 +433,12 @@ __global__ __launch_bounds__(256, T == 64 ? 3 : 2) void k_ns_gemm(Mats M, Part p
         for (int kk = 0; kk < 2; kk++) {
             __builtin_amdgcn_s_setprio(1);  // the wave that multiplies goes first: 3 % of a 4096 x 4096 product
 #pragma unroll
-            for (int pr = NP == 3 ? 0 : 2; pr < 3; pr++)  // lo hi, hi lo, hi hi; the same accumulator again only after W W others
+            for (int pr = 0; pr < 3; pr++)  // lo hi, hi lo, hi hi; the same accumulator again only after W W others
 #pragma unroll
                 for (int x = 0; x < W; x++)
 #pragma unroll
                     for (int y = 0; y < W; y++)
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][pr == 0 ? NPL - 1 : 0][x], fq[kk][pr == 1 ? NPL - 1 : 0][y], acc[x][y], 0, 0, 0);
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[kk][pr == 0][x], fq[kk][pr == 1][y], acc[x][y], 0, 0, 0);
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
             if (kk == 0) place(st ^ 1, rp[(d + 1) % D], rq[(d + 1) % D]);
@@ -1006,10 +1002,6 @@ int path_of(int64_t rows, int64_t cols) {
 }
 // Matrices whose shorter side is 512 or more are padded so that tiles of 128 may be used.
 int pad_of(int64_t rows, int64_t cols) { return (rows < cols ? rows : cols) >= 512 ? 128 : 64; }
-bool one_product(const OrthoMatrix& q, const OrthoStep& o) {
-    const int64_t s = q.rows < q.cols ? q.rows : q.cols, l = q.rows < q.cols ? q.cols : q.rows;
-    return !o.muon && o.dtype == 1 && s >= 1024 && s * s >= 256 * l;
-}
 
 int64_t layout(const OrthoMatrix& q, char* base, Mat* m) {
     const int64_t s = q.rows < q.cols ? q.rows : q.cols, l = q.rows < q.cols ? q.cols : q.rows;
@@ -1062,7 +1054,7 @@ int set_starts(Mats& M, int T, int kc) {
     }
     return wgs;
 }
-template <int NP, int KIND, int T>
+template <int KIND, int T>
 void run_symmetric(Mats& M, int tiles, float* partial, int odd, int last, hipStream_t s) {
     constexpr int D = T == 64 ? 4 : 2;
     int64_t stages = 0;
@@ -1075,16 +1067,16 @@ void run_symmetric(Mats& M, int tiles, float* partial, int odd, int last, hipStr
     int kc = (int)((stages + SPLIT_GOAL - 1) / SPLIT_GOAL);
     if (kc < SPLIT_MIN) kc = SPLIT_MIN;
     if (tiles >= SPLIT_BELOW || longest < 3 * kc) {
-        hipLaunchKernelGGL((k_ns_gemm<T, NP, KIND, D>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
+        hipLaunchKernelGGL((k_ns_gemm<T, KIND, D>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
         return;
     }
     const Part part = {0, 0, odd, last, kc, partial};
     const int wgs = set_starts<KIND>(M, T, kc);
-    hipLaunchKernelGGL((k_ns_gemm<T, NP, KIND, D>), dim3(wgs), dim3(256), 0, s, M, part);
+    hipLaunchKernelGGL((k_ns_gemm<T, KIND, D>), dim3(wgs), dim3(256), 0, s, M, part);
     set_starts<KIND>(M, T, 0);
     hipLaunchKernelGGL((k_ns_join<T, KIND>), dim3(tiles, T * T / 1024), dim3(256), 0, s, M, part);
 }
-template <int NP, int KIND>
+template <int KIND>
 void run_gemm(Mats& M, bool may128, float* partial, int odd, int last, hipStream_t s) {
     int tiles = may128 ? set_starts<KIND>(M, 128, 0) : 0;
     // Tiles of 128 read half as much through LDS per product, tiles of 64 give four times the workgroups.  B = b A + c A A, whose sum is
@@ -1093,25 +1085,24 @@ void run_gemm(Mats& M, bool may128, float* partial, int odd, int last, hipStream
     // tiles of 64, 33 us in tiles of 128 split along the sum).
     if (tiles < (KIND == KIND_POLY ? 128 : 32)) {
         tiles = set_starts<KIND>(M, 64, 0);
-        if (KIND == KIND_APPLY) hipLaunchKernelGGL((k_ns_gemm<64, NP, KIND, 4>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
-        else run_symmetric<NP, KIND, 64>(M, tiles, partial, odd, last, s);
+        if (KIND == KIND_APPLY) hipLaunchKernelGGL((k_ns_gemm<64, KIND, 4>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
+        else run_symmetric<KIND, 64>(M, tiles, partial, odd, last, s);
         return;
     }
     if (KIND != KIND_APPLY && tiles <= SLOTS) {
-        run_symmetric<NP, KIND, 128>(M, tiles, partial, odd, last, s);
+        run_symmetric<KIND, 128>(M, tiles, partial, odd, last, s);
         return;
     }
     // what is left over a multiple of the slots runs in quarters, if it is less than half a round
     const int rest = tiles % SLOTS, head = tiles > SLOTS && rest * 2 < SLOTS ? tiles - rest : tiles;
-    hipLaunchKernelGGL((k_ns_gemm<128, NP, KIND, 2>), dim3(head), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
-    if (head < tiles) hipLaunchKernelGGL((k_ns_gemm<64, NP, KIND, 4>), dim3(4 * (tiles - head)), dim3(256), 0, s, M, Part{head, 1, odd, last, 0, nullptr});
+    hipLaunchKernelGGL((k_ns_gemm<128, KIND, 2>), dim3(head), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
+    if (head < tiles) hipLaunchKernelGGL((k_ns_gemm<64, KIND, 4>), dim3(4 * (tiles - head)), dim3(256), 0, s, M, Part{head, 1, odd, last, 0, nullptr});
 }
-template <int NP>
 hipError_t run_steps(Mats& M, bool may128, float* partial, hipStream_t s) {
     for (int step = 0; step < M.o.steps; step++) {
-        run_gemm<NP, KIND_GRAM>(M, may128, partial, step & 1, 0, s);
-        run_gemm<NP, KIND_POLY>(M, may128, partial, step & 1, 0, s);
-        run_gemm<NP, KIND_APPLY>(M, may128, partial, step & 1, step + 1 == M.o.steps, s);
+        run_gemm<KIND_GRAM>(M, may128, partial, step & 1, 0, s);
+        run_gemm<KIND_POLY>(M, may128, partial, step & 1, 0, s);
+        run_gemm<KIND_APPLY>(M, may128, partial, step & 1, step + 1 == M.o.steps, s);
     }
     return hipGetLastError();
 }
@@ -1157,7 +1148,7 @@ hipError_t run_strips(Mats& M, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t run_group(Mats& M, int pad, bool one, float* partial, hipStream_t s) {
+hipError_t run_group(Mats& M, int pad, float* partial, hipStream_t s) {
     int wgs = 0;
     for (int i = 0; i < M.count; i++) {
         M.start[i] = wgs;
@@ -1170,7 +1161,7 @@ hipError_t run_group(Mats& M, int pad, bool one, float* partial, hipStream_t s) 
         wgs += (M.m[i].sp >> 6) * (M.m[i].lp >> 6);
     }
     hipLaunchKernelGGL(k_ns_split, dim3(wgs), dim3(256), 0, s, M);
-    return one ? run_steps<1>(M, pad == 128, partial, s) : run_steps<3>(M, pad == 128, partial, s);
+    return run_steps(M, pad == 128, partial, s);
 }
 
 // Room for the partial sums of split products: a launch has at most SPLIT_GOAL pieces and one more per tile (the last of each), and no
@@ -1202,24 +1193,24 @@ int64_t ortho_workspace_bytes(const OrthoMatrix* q, int count, const OrthoStep&)
 }
 
 hipError_t orthogonalize(const OrthoMatrix* q, int count, const OrthoStep& o, void* ws, hipStream_t s) {
-    // groups that share their launches: strips and tiny ones, and tiles of either padding and precision
+    // groups that share their launches: strips and tiny ones, and tiles of either padding
     float* partial = static_cast<float*>(ws);
-    for (int group = 0; group < 5; group++) {
-        const bool tiles = group > 0, one = tiles && (group - 1) & 1;
-        const int pad = group <= 2 ? 64 : 128;
+    for (int group = 0; group < 3; group++) {
+        const bool tiles = group > 0;
+        const int pad = group == 1 ? 64 : 128;
         Mats M;
         M.o = o;
         M.count = 0;
         char* base = static_cast<char*>(ws) + partial_bytes(q, count);
         auto run = [&]() -> hipError_t {
-            const hipError_t e = tiles ? run_group(M, pad, one, partial, s) : run_strips(M, s);
+            const hipError_t e = tiles ? run_group(M, pad, partial, s) : run_strips(M, s);
             M.count = 0;
             return e;
         };
         for (int i = 0; i < count; i++) {
             if (q[i].rows <= 0 || q[i].cols <= 0) continue;
             const bool in_tiles = path_of(q[i].rows, q[i].cols) == PATH_TILES;
-            if (in_tiles == tiles && (!tiles || (pad_of(q[i].rows, q[i].cols) == pad && one_product(q[i], o) == one))) {
+            if (in_tiles == tiles && (!tiles || pad_of(q[i].rows, q[i].cols) == pad)) {
                 Mat m;
                 layout(q[i], base, &m);
                 // longest first: their workgroups run longest; tiny ones at the end
