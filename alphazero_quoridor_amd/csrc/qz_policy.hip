@@ -201,6 +201,8 @@ __device__ __forceinline__ float series2(float x) {
 __device__ __forceinline__ float expm1_minus_x(float x) {  // e^x - 1 - x >= 0
     return fabsf(x) < 0.5f ? series2(x) * x * x : expf(x) - 1.f - x;
 }
+// e^x - 1, the derivative of that: by itself, since adding x back to it gives inf - inf where x = -inf, and 0 for -1 past 2^24
+__device__ __forceinline__ float expm1_near(float x) { return fabsf(x) < 0.5f ? series2(x) * x * x + x : expf(x) - 1.f; }
 __device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, int64_t act, float za, const Stat& st, const Stat& sq, float scale) {
     RowOut o;
     const float h = stat_entropy(st);
@@ -217,9 +219,9 @@ __device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, i
     float c = held_wins ? 0.f : -open;
     o.loss = held_wins ? -held : -open;
     if (P.ref_logp) {
-        const float x = P.ref_logp[row] - o.logp, f = expm1_minus_x(x);
-        o.loss += P.kl_coef * f;
-        c -= P.kl_coef * (f + x);
+        const float x = P.ref_logp[row] - o.logp;
+        o.loss += P.kl_coef * expm1_minus_x(x);
+        c -= P.kl_coef * expm1_near(x);
     }
     o.loss -= P.entropy_coef * h;
     const bool on = w != 0.f;

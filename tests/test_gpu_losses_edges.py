@@ -1,0 +1,42 @@
+"""Policy losses (losses.py, csrc/qz_policy.hip) where a frozen policy forbids what the other one does, in every form that a row's width
+and number choose, against the definitions in float64.  Definitions and tolerances: tests/test_gpu_losses.py."""
+import math
+
+import pytest
+import torch
+from test_gpu_losses import close, definition, grad_tolerance, make, pack, stored
+
+pytestmark = pytest.mark.gpu
+
+# a wave per row; a workgroup per row in registers, of 256 and of 1,024; read twice; few rows split over workgroups
+FORMS = ((5, 140, torch.float32, "bits"), (5, 3000, torch.bfloat16, "none"), (5, 50001, torch.bfloat16, "bytes"), (70, 66003, torch.float16, "none"), (5, 70000, torch.float32, "none"))
+
+
+def call(d, device, kind, kl, kl_coef, ent_coef=0.02, **kw):
+    """-> (result, gradient) through autograd, after the same through policy_loss_and_grad"""
+    from alphazero_quoridor_amd import losses
+
+    dev = {k: v.to(device) for k, v in d.items()}
+    legal = None if kind == "none" else dev["legal"] if kind == "bytes" else pack(d["legal"]).to(device)
+    args = dict(legal=legal, weights=dev["w"], ref_logits=dev["ref"] if kl == "full" else None, ref_logp=dev["ref_logp"] if kl == "taken" else None,
+                kl_coef=kl_coef, entropy_coef=ent_coef, **kw)
+    z = dev["z"].clone().requires_grad_(True)
+    out = losses.clipped_policy_loss(z, dev["actions"], dev["adv"], dev["old"], **args)
+    out.loss.backward()
+    raw, grad = losses.policy_loss_and_grad(dev["z"], dev["actions"], dev["adv"], dev["old"], **args)
+    assert torch.equal(grad, z.grad) and torch.equal(raw.logp, out.logp)
+    return out, z.grad
+
+
+@pytest.mark.parametrize("n,a,dtype,kind", FORMS, ids=str)
+def test_a_frozen_policy_that_forbids_the_action_taken(gpu_device, n, a, dtype, kind):
+    """KL estimated from ref_logp = -inf, or a mask's lowest value: an infinite or huge term, whose gradient is that of -x: the
+    derivative e^x - 1 of e^x - 1 - x is -1 there."""
+    d = make(n, a, dtype, 17 + a)
+    d["ref_logp"][:5] = torch.tensor([-math.inf, -torch.finfo(torch.float32).max, -1e9, -3e7, -2.0])
+    e = definition(d, kind != "none", "taken", (0.2, 0.2), 0.05, 0.02)
+    assert torch.isfinite(e["grad"]).all()
+    out, grad = call(d, gpu_device, kind, "taken", 0.05)
+    close(out.kl, e["kl"], e["kl_tol"], "kl")
+    assert float(out.loss.detach()) == math.inf
+    close(grad, stored(e["grad"], dtype), grad_tolerance(e, dtype), "grad")
