@@ -218,7 +218,7 @@ __device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, i
     const bool held_wins = held < open;
     float c = held_wins ? 0.f : -open;
     o.loss = held_wins ? -held : -open;
-    if (P.ref_logp) {
+    if (P.ref_logp && P.kl_coef != 0.f) {  // (a factor of 0: an infinite KL takes no part)
         const float x = P.ref_logp[row] - o.logp;
         o.loss += P.kl_coef * expm1_minus_x(x);
         c -= P.kl_coef * expm1_near(x);
@@ -235,6 +235,10 @@ __device__ __forceinline__ RowOut row_terms(const PolicyTerms& P, int64_t row, i
     o.g.on = on;
     return o;
 }
+// what KL over the frozen policy's logits adds to the loss: nothing where a factor is 0, infinite or NaN as it may be
+__device__ __forceinline__ double kl_part(const PolicyTerms& P, bool live, float w, float kl) {
+    return P.ref_logits && live && w != 0.f && P.kl_coef != 0.f ? (double)w * P.kl_coef * kl : 0.0;
+}
 __device__ __forceinline__ float kl_taken(const PolicyTerms& P, int64_t row, float logp) { return P.ref_logp ? expm1_minus_x(P.ref_logp[row] - logp) : 0.f; }
 
 // one column: gradient, and the column's term of KL over logits.  p = 0 (a logit of -inf) gives 0 log 0 = 0; q = 0 < p has no KL
@@ -248,7 +252,7 @@ __device__ __forceinline__ float column(const Coef& g, bool has_q, float z, floa
         const float x = (dz - dq) - (g.ls - g.lsq);
         const float f = fabsf(x) < 0.5f ? q * (series2(x) * x * x) : q == 0.f ? p : (p - q) - q * x;
         kl += f;
-        d += g.beta * (p - q);
+        if (g.beta != 0.f) d += g.beta * (p - q);
     }
     if (j == g.act) d += g.c;
     return g.on ? d : 0.f;
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
         O.logp[row] = o.logp;
         O.kl[row] = live ? kl : 0.f;
         O.entropy[row] = h;
-        O.parts[row] = (double)o.loss + (P.ref_logits && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+        O.parts[row] = (double)o.loss + kl_part(P, live, w, kl);
     }
 }
 
@@ -754,7 +758,7 @@ __global__ __launch_bounds__(256) void k_wave_loss(PolicyRows R, PolicyTerms P, 
         O.logp[row] = o.logp;
         O.kl[row] = live ? kl : 0.f;
         O.entropy[row] = h;
-        O.parts[row] = (double)o.loss + (has_q && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+        O.parts[row] = (double)o.loss + kl_part(P, live, w, kl);
     }
 }
 
@@ -928,7 +932,7 @@ __global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P,
         O.logp[row] = o.logp;
         O.kl[row] = live ? kl : 0.f;
         O.entropy[row] = h;
-        O.parts[row] = (double)o.loss + (HAS_Q && live && w != 0.f ? (double)w * P.kl_coef * kl : 0.0);
+        O.parts[row] = (double)o.loss + kl_part(P, live, w, kl);
     }
 }
 

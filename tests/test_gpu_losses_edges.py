@@ -40,3 +40,25 @@ def test_a_frozen_policy_that_forbids_the_action_taken(gpu_device, n, a, dtype, 
     close(out.kl, e["kl"], e["kl_tol"], "kl")
     assert float(out.loss.detach()) == math.inf
     close(grad, stored(e["grad"], dtype), grad_tolerance(e, dtype), "grad")
+
+
+@pytest.mark.parametrize("kl", ("taken", "full"))
+@pytest.mark.parametrize("n,a,dtype,kind", FORMS, ids=str)
+def test_a_term_with_the_factor_zero_takes_no_part(gpu_device, n, a, dtype, kind, kl):
+    """kl_coef = 0 only watches KL: where it is infinite (or, a legal frozen logit being NaN, undefined), loss and gradient are those
+    without a frozen policy."""
+    d = make(n, a, dtype, 23 + a)
+    d["ref_logp"][0] = -math.inf
+    other = (d["actions"] + 1) % a  # legal, and given no probability by the policy in row 1, none by the frozen one in row 2
+    d["legal"][torch.arange(n), other] = True
+    d["z"][1, other[1]] = -math.inf
+    d["ref"][2, other[2]] = -math.inf
+    d["ref"][3, other[3]] = math.nan
+    e = definition(d, kind != "none", "none", (0.2, 0.2), 0.0, 0.02)
+    out, grad = call(d, gpu_device, kind, kl, 0.0)
+    assert math.isinf(float(out.kl[0 if kl == "taken" else 1]))
+    assert kl == "taken" or math.isnan(float(out.kl[3]))
+    close(out.loss.detach(), e["loss"], e["loss_tol"], "loss")
+    close(out.logp, e["logp"], e["logp_tol"], "logp")
+    close(out.entropy, e["entropy"], e["entropy_tol"], "entropy")
+    close(grad, e["grad"], grad_tolerance(e, dtype), "grad")
