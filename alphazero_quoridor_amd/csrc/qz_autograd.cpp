@@ -18,6 +18,12 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasquerad
 void check(int rc) { TORCH_CHECK(rc == 0, "libqzero_hip error ", rc, ": ", qz_last_error()); }
 // a backward pass under create_graph would return a gradient that autograd takes for a constant
 void refuse_twice() { TORCH_CHECK(!at::GradMode::is_enabled(), "the policy losses can be differentiated once only (create_graph is not supported)"); }
+// A dual tensor requires no gradient, so the functions below would compute on its values and drop its tangent without a word.
+void refuse_tangents(std::initializer_list<Tensor> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "the policy losses have no forward-mode derivative");
+}
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? QZ_F32 : t.scalar_type() == at::kBFloat16 ? QZ_BF16 : QZ_F16; }
@@ -99,6 +105,7 @@ struct ActionLogp : torch::autograd::Function<ActionLogp> {
 };
 std::tuple<Tensor, Tensor> action_logp(const Tensor& z, const Tensor& actions, const std::optional<Tensor>& legal, int64_t kind, bool entropy) {
     const Tensor mask = legal.value_or(Tensor());
+    refuse_tangents({z});
     if (at::GradMode::is_enabled() && z.requires_grad()) {
         const variable_list out = ActionLogp::apply(z, LogpArgs{actions, mask, kind, entropy});
         return {out[0], entropy ? out[1] : Tensor()};
@@ -173,6 +180,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Maybe> policy_loss(const Tensor& z, c
                                                               const Tensor& old_logp, const Maybe& ref_logp, const Maybe& weights, const Maybe& ref, double lo,
                                                               double hi, double kl, double ent, bool raw_grad) {
     const LossArgs a = {actions, legal.value_or(Tensor()), adv, old_logp, ref_logp.value_or(Tensor()), weights.value_or(Tensor()), ref.value_or(Tensor()), kind, lo, hi, kl, ent};
+    refuse_tangents({z, adv, old_logp, a.ref_logp, a.weights, a.ref});
     if (!raw_grad && at::GradMode::is_enabled() && z.requires_grad()) {
         const variable_list o = PolicyLoss::apply(z, a);
         return {o[0], o[1], o[2], o[3], Maybe()};

@@ -8,7 +8,8 @@ logits too).  ``legal`` is None, a mask of bytes or bools [..., A], or packed 32
 has a logit of -inf is left out: no loss, no gradient, no entropy; its log-probability reads 0 for a negative action (padding)
 and -inf otherwise.  Illegal columns may hold anything, NaN included.
 
-There is no CPU path: tensors on another device than a GPU raise ``QzError(QZ_E_NO_DEVICE)``."""
+Derivatives are reverse-mode and first-order: a second derivative and forward-mode tangents are refused (RuntimeError,
+NotImplementedError).  There is no CPU path: tensors on another device than a GPU raise ``QzError(QZ_E_NO_DEVICE)``."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional

@@ -62,3 +62,31 @@ def test_a_term_with_the_factor_zero_takes_no_part(gpu_device, n, a, dtype, kind
     close(out.logp, e["logp"], e["logp_tol"], "logp")
     close(out.entropy, e["entropy"], e["entropy_tol"], "entropy")
     close(grad, e["grad"], grad_tolerance(e, dtype), "grad")
+
+
+def test_forward_mode_is_refused(gpu_device):
+    """A dual tensor requires no gradient: its tangent must not be dropped in silence, in the logits or in what is constant otherwise."""
+    import torch.autograd.forward_ad as fwd
+    from alphazero_quoridor_amd import losses
+
+    d = {k: v.to(gpu_device) for k, v in make(6, 20, torch.float32, 1).items()}
+
+    def both(**change):
+        a = dict(dict(logits=d["z"], actions=d["actions"], advantages=d["adv"], old_logp=d["old"]), **change)
+        return (lambda: losses.clipped_policy_loss(**a)), (lambda: losses.policy_loss_and_grad(**a))
+
+    want = losses.clipped_policy_loss(d["z"], d["actions"], d["adv"], d["old"]).loss
+    with fwd.dual_level():
+        calls = []
+        for name, key in (("logits", "z"), ("advantages", "adv"), ("old_logp", "old"), ("weights", "w"), ("ref_logits", "ref"), ("ref_logp", "ref_logp")):
+            calls += both(**{name: fwd.make_dual(d[key], torch.ones_like(d[key]))})
+        dual = fwd.make_dual(d["z"], torch.ones_like(d["z"]))
+        calls += [lambda: losses.action_logp(dual, d["actions"]), lambda: losses.action_logp(dual.view(2, 3, 20), d["actions"].view(2, 3), entropy=True),
+                  lambda: losses.action_logp(dual.clone().requires_grad_(True) * 1, d["actions"])]
+        for k, f in enumerate(calls):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+                pytest.fail("call %d went through" % k)
+        primal = fwd.unpack_dual(dual).primal
+        assert torch.equal(losses.clipped_policy_loss(primal, d["actions"], d["adv"], d["old"]).loss, want)
+    assert torch.equal(losses.clipped_policy_loss(d["z"], d["actions"], d["adv"], d["old"]).loss, want)
