@@ -9,6 +9,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 from .losses import DTYPES, _call, _gpu
@@ -39,11 +40,19 @@ def _float_word(v):
     return struct.unpack("q", struct.pack("fi", v, 0))[0]
 
 
-@torch.no_grad()
+def _constant(t, name):
+    """The result carries no derivative: an input that asks for one is refused."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires grad, but the result is a constant: detach it" % name)
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError("%s: orthogonalisation has no forward-mode derivative" % name)
+
+
 def orthogonalize(update, steps=5):
     """The Newton-Schulz iterate of ``update`` / |update|_F after ``steps`` (1 .. 16) quintic steps: same singular vectors, singular
     values near 1.  A tensor [rows, ...] (trailing dimensions count as columns), or a list of them, which share their launches.
-    float32, bfloat16 or float16; the result has the type and shape of its input."""
+    float32, bfloat16 or float16; the result has the type and shape of its input.  Not differentiable: an update that requires grad is
+    refused (outside torch.no_grad()), and so is one with a forward-mode tangent."""
     many = isinstance(update, (list, tuple))
     updates = list(update) if many else [update]
     steps = int(steps)
@@ -51,7 +60,9 @@ def orthogonalize(update, steps=5):
         raise ValueError("steps = %d is not in 1 .. 16" % steps)
     outs, batches, keep = [], {}, []
     for u in updates:
-        m = _matrix(u, "update")
+        _gpu(u, "update")
+        _constant(u, "update")
+        m = _matrix(u.detach(), "update")
         if u.dtype not in DTYPES:
             raise TypeError("update: %s is not one of float32, bfloat16, float16" % u.dtype)
         o = torch.empty(u.shape, dtype=u.dtype, device=u.device)
