@@ -598,6 +598,11 @@ class PolicyValueNet:
         logp, v = self.policy_value_net(states)
         return torch.exp(logp), v
 
+    @torch.no_grad()
+    def log_policy_value_t(self, states: torch.Tensor):
+        """policy_value_t with the log-probabilities themselves: (log_act_probs [B,140], value [B,1])."""
+        return self.policy_value_net(states)
+
     def train_step_t(self, states, mcts_probs, winners, lr):
         """One optimiser step on device tensors (policy_value_net.py:166-192):
         loss = mse(v, z) - mean(sum(pi * log p)) (+ L2 through Adam's weight decay).  Returns

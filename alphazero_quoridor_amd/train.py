@@ -206,13 +206,15 @@ class TrainPipeline(object):
         else:
             boards, pi, z = self.data_buffer.gather(self.data_buffer.sample_indices(self.batch_size))
             states, legal = rules.encode(boards), rules.movegen(boards)
-        old_probs, old_v = net.policy_value_t(states)
-        old_logp = torch.log(old_probs + 1e-10)
+        net_logp, old_v = net.log_policy_value_t(states)
+        old_probs = torch.exp(net_logp)
+        old_logp = torch.log(old_probs + 1e-10)  # (the reference's, for the KL that controls the step)
         if self.objective == "clipped":
-            # a move of the search's distribution, its log-probability among the legal ones before the update, and how much better the
-            # game ended than the net had expected
+            # a move of the search's distribution, its log-probability among the legal ones before the update (the net's own: with 1e-10
+            # added, a move it holds below that would start at a ratio near 0 instead of 1), and how much better the game ended than
+            # the net had expected
             moves = torch.multinomial(pi, 1).view(-1)
-            move_logp, advantages = losses.action_logp(old_logp, moves, legal=legal), z - old_v.view(-1)
+            move_logp, advantages = losses.action_logp(net_logp, moves, legal=legal), z - old_v.view(-1)
         loss = entropy = None
         new_v = old_v
         kl = 0.0
@@ -222,7 +224,7 @@ class TrainPipeline(object):
             if self.objective == "mcts":
                 loss, entropy = net.train_step_t(states, pi, z, lr)
             else:
-                loss, entropy = net.policy_step_t(states, moves, advantages, move_logp, z, lr, legal=legal, ref_logits=old_logp, clip=self.clip,
+                loss, entropy = net.policy_step_t(states, moves, advantages, move_logp, z, lr, legal=legal, ref_logits=net_logp, clip=self.clip,
                                                   kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
             new_probs, new_v = net.policy_value_t(states)
             kl_t = torch.mean(torch.sum(old_probs * (old_logp - torch.log(new_probs + 1e-10)), dim=1))
