@@ -13,6 +13,7 @@ struct PolicyRows {
     int32_t legal_kind;
     int32_t dtype;           // 0 float32, 1 bfloat16, 2 float16
     int32_t a;
+    int64_t row0 = 0;        // first row of a launch
 };
 struct PolicyTerms {
     const float *advantages, *old_logp, *ref_logp, *weights;  // [n]; ref_logp, weights may be null

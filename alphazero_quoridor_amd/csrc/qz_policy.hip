@@ -477,7 +477,7 @@ __device__ __forceinline__ Stat row_stat(const PolicyRows& R, const void* base, 
 template <typename T, int RT>
 __global__ __launch_bounds__(RT) void k_action_logp(PolicyRows R, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
     __shared__ float sh[3 * RT / 64];
-    const int64_t row = blockIdx.x;
+    const int64_t row = R.row0 + blockIdx.x;
     int64_t act;
     float za;
     const bool live = row_live<T>(R, row, act, za);
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(BT) void k_action_logp_backward(PolicyRows R, const
                                                              const float* __restrict__ dlogp, const float* __restrict__ dentropy, void* __restrict__ grad,
                                                              int64_t ld_grad) {
     constexpr int V = Elem<T>::V;
-    const int64_t row = blockIdx.x;
+    const int64_t row = R.row0 + blockIdx.x;
     int64_t act;
     float za;
     const bool live = row_live<T>(R, row, act, za);
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(RT) void k_policy_loss(PolicyRows R, PolicyTerms P,
     __shared__ float sh[3 * RT / 64];
     const float scale = O.scale ? *O.scale : 1.f;
     if (O.only_if_scaled && scale == 1.f) return;  // the gradient that the forward pass wrote is the one asked for
-    const int64_t row = blockIdx.x;
+    const int64_t row = R.row0 + blockIdx.x;
     int64_t act;
     float za;
     const bool live = row_live<T>(R, row, act, za);
@@ -696,7 +696,7 @@ __device__ __forceinline__ Stat wave_stat(const float (&z)[E]) {
 template <typename T, int E>
 __global__ __launch_bounds__(256) void k_wave_logp(PolicyRows R, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t row = R.row0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= R.n) return;
     float z[E];
 #pragma unroll
@@ -720,7 +720,7 @@ __global__ __launch_bounds__(256) void k_wave_loss(PolicyRows R, PolicyTerms P, 
     const float scale = O.scale ? *O.scale : 1.f;
     if (O.only_if_scaled && scale == 1.f) return;
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t row = R.row0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= R.n) return;
     const bool has_q = P.ref_logits != nullptr;
     float z[E], zq[E];
@@ -825,7 +825,7 @@ __global__ __launch_bounds__(NT, 4) void k_row_loss(PolicyRows R, PolicyTerms P,
     __shared__ float sh[3][48];
     const float scale = O.scale ? *O.scale : 1.f;
     if (O.only_if_scaled && scale == 1.f) return;
-    const int64_t row = blockIdx.x;
+    const int64_t row = R.row0 + blockIdx.x;
     const T* zrow = static_cast<const T*>(R.logits) + row * R.ld;
     const T* qrow = static_cast<const T*>(P.ref_logits) + row * P.ref_ld;
     const int j0 = threadIdx.x * V, full = R.a / V * V, jt = full + threadIdx.x;
@@ -967,9 +967,16 @@ constexpr int WAVE_WIDEST = 1024, WAVE_WIDEST_LOSS = 512;
     else if ((a) <= 192) { constexpr int E = 3; __VA_ARGS__; } \
     else { constexpr int E = 8; __VA_ARGS__; }
 
+// launch(rows from R.row0 on, workgroups) for all rows, `per` of them to a workgroup.  A launch takes fewer than 2^32 work-items a
+// dimension, so 2^21 workgroups of up to 1,024; more rows (17 million of two columns are 134 MB) go to further launches.
+template <typename F>
+void by_rows(PolicyRows R, int per, F launch) {
+    const int64_t most = (int64_t)(1 << 21) * per;
+    for (R.row0 = 0; R.row0 < R.n; R.row0 += most) launch(R, (unsigned)(((R.n - R.row0 < most ? R.n - R.row0 : most) + per - 1) / per));
+}
 template <typename T, int NT, int CH>
-void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
-    const dim3 grid((unsigned)R.n), block(NT);
+void row_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, unsigned wgs, hipStream_t s) {
+    const dim3 grid(wgs), block(NT);
     if (P.ref_logits && R.legal_kind) hipLaunchKernelGGL((k_row_loss<T, NT, CH, true, true>), grid, block, 0, s, R, P, O);
     else if (P.ref_logits) hipLaunchKernelGGL((k_row_loss<T, NT, CH, true, false>), grid, block, 0, s, R, P, O);
     else if (R.legal_kind) hipLaunchKernelGGL((k_row_loss<T, NT, CH, false, true>), grid, block, 0, s, R, P, O);
@@ -983,16 +990,16 @@ bool few(int64_t n) { return n <= 256; }
 // a CU to itself, and nothing to cover its loads with (2,048 x 50,001: 315 us, 226 us read twice) -- but for one input with a mask, whose
 // second reading costs more (2,047 x 50,001 with a byte mask: 180 us, 191 us read twice).
 template <typename T>
-void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, hipStream_t s) {
+void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, unsigned wgs, hipStream_t s) {
     const int chunks = (R.a + Elem<T>::V - 1) / Elem<T>::V;
-    if (chunks <= 256) row_loss<T, 256, 1>(R, P, O, s);
-    else if (chunks <= 512) row_loss<T, 256, 2>(R, P, O, s);
-    else if (chunks <= 1024) row_loss<T, 256, 4>(R, P, O, s);
-    else if (chunks <= 2048) row_loss<T, 512, 4>(R, P, O, s);
-    else if (chunks <= 4096) row_loss<T, 512, 8>(R, P, O, s);
-    else if (chunks <= 8192 && R.legal_kind && !P.ref_logits) hipLaunchKernelGGL((k_row_loss<T, 1024, 8, false, true>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
-    else if (few(R.n)) hipLaunchKernelGGL((k_policy_loss<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, P, O);
-    else hipLaunchKernelGGL((k_policy_loss<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, P, O);
+    if (chunks <= 256) row_loss<T, 256, 1>(R, P, O, wgs, s);
+    else if (chunks <= 512) row_loss<T, 256, 2>(R, P, O, wgs, s);
+    else if (chunks <= 1024) row_loss<T, 256, 4>(R, P, O, wgs, s);
+    else if (chunks <= 2048) row_loss<T, 512, 4>(R, P, O, wgs, s);
+    else if (chunks <= 4096) row_loss<T, 512, 8>(R, P, O, wgs, s);
+    else if (chunks <= 8192 && R.legal_kind && !P.ref_logits) hipLaunchKernelGGL((k_row_loss<T, 1024, 8, false, true>), dim3(wgs), dim3(1024), 0, s, R, P, O);
+    else if (few(R.n)) hipLaunchKernelGGL((k_policy_loss<T, 1024>), dim3(wgs), dim3(1024), 0, s, R, P, O);
+    else hipLaunchKernelGGL((k_policy_loss<T, 256>), dim3(wgs), dim3(256), 0, s, R, P, O);
 }
 }  // namespace
 
@@ -1023,9 +1030,10 @@ int64_t policy_workspace_bytes(int64_t n, int a) { return n * 8 + (few_wide(n, a
 hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* stats, void* ws, hipStream_t s) {
     if (R.n <= 0) return hipSuccess;
     if (R.a > 512 && R.a <= WAVE_WIDEST) {
-        BY_TYPE(R.dtype, hipLaunchKernelGGL((k_wave_logp<T, 16>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats));
+        BY_TYPE(R.dtype, by_rows(R, 4, [&](const PolicyRows& Q, unsigned wgs) { hipLaunchKernelGGL((k_wave_logp<T, 16>), dim3(wgs), dim3(256), 0, s, Q, logp, entropy, stats); }));
     } else if (R.a <= 512) {
-        BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_logp<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, logp, entropy, stats)));
+        BY_TYPE(R.dtype, BY_WIDTH(R.a, by_rows(R, 4, [&](const PolicyRows& Q, unsigned wgs) {
+                    hipLaunchKernelGGL((k_wave_logp<T, E>), dim3(wgs), dim3(256), 0, s, Q, logp, entropy, stats); })));
     } else if (few_wide(R.n, R.a)) {
         const PolicyTerms none = {};
         BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws);
@@ -1034,7 +1042,7 @@ hipError_t action_logp(const PolicyRows& R, float* logp, float* entropy, float* 
     } else if (few(R.n) && R.a >= 65536) {  // (shorter rows: four waves, 1,024 x 8,192 8 us, and 22 us with sixteen)
         BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 1024>), dim3((unsigned)R.n), dim3(1024), 0, s, R, logp, entropy, stats));
     } else {
-        BY_TYPE(R.dtype, hipLaunchKernelGGL((k_action_logp<T, 256>), dim3((unsigned)R.n), dim3(256), 0, s, R, logp, entropy, stats));
+        BY_TYPE(R.dtype, by_rows(R, 1, [&](const PolicyRows& Q, unsigned wgs) { hipLaunchKernelGGL((k_action_logp<T, 256>), dim3(wgs), dim3(256), 0, s, Q, logp, entropy, stats); }));
     }
     return hipGetLastError();
 }
@@ -1043,14 +1051,15 @@ hipError_t action_logp_backward(const PolicyRows& R, const float* stats, const f
     if (R.n <= 0) return hipSuccess;
     // few rows: several workgroups for each, up to one per pass over BT chunks
     BY_TYPE(R.dtype, const int most = (R.a + BT * Elem<T>::V - 1) / (BT * Elem<T>::V); int y = (int)((1024 + R.n - 1) / R.n); y = y < most ? y : most;
-            hipLaunchKernelGGL((k_action_logp_backward<T>), dim3((unsigned)R.n, y), dim3(BT), 0, s, R, stats, entropy, dlogp, dentropy, grad, ld_grad));
+            by_rows(R, 1, [&](const PolicyRows& Q, unsigned wgs) {
+                hipLaunchKernelGGL((k_action_logp_backward<T>), dim3(wgs, y), dim3(BT), 0, s, Q, stats, entropy, dlogp, dentropy, grad, ld_grad); }));
     return hipGetLastError();
 }
 hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, float* loss, void* ws, hipStream_t s) {
     O.parts = loss ? static_cast<double*>(ws) : nullptr;
     if (R.n > 0) {
         if (R.a <= WAVE_WIDEST_LOSS) {
-            BY_TYPE(R.dtype, BY_WIDTH(R.a, hipLaunchKernelGGL((k_wave_loss<T, E>), dim3((unsigned)((R.n + 3) / 4)), dim3(256), 0, s, R, P, O)));
+            BY_TYPE(R.dtype, BY_WIDTH(R.a, by_rows(R, 4, [&](const PolicyRows& Q, unsigned wgs) { hipLaunchKernelGGL((k_wave_loss<T, E>), dim3(wgs), dim3(256), 0, s, Q, P, O); })));
         } else if (few_wide(R.n, R.a)) {
             BY_TYPE(R.dtype, const Split S = make_split(R.n, R.a, Elem<T>::V, ws); const dim3 grid(S.s, (unsigned)R.n);
                     hipLaunchKernelGGL((k_split_stats<T>), grid, dim3(ST), 0, s, R, P, S, O.scale, O.only_if_scaled);
@@ -1058,7 +1067,7 @@ hipError_t policy_loss(const PolicyRows& R, const PolicyTerms& P, PolicyOut O, f
                     if (loss) hipLaunchKernelGGL(k_split_finish, dim3(1), dim3(256), 0, s, O, S, (int)R.n, P.ref_logits != nullptr, loss));
             return hipGetLastError();
         } else {
-            BY_TYPE(R.dtype, wide_loss<T>(R, P, O, s));
+            BY_TYPE(R.dtype, by_rows(R, 1, [&](const PolicyRows& Q, unsigned wgs) { wide_loss<T>(Q, P, O, wgs, s); }));
         }
     }
     if (loss) hipLaunchKernelGGL(k_sum_parts, dim3(1), dim3(1024), 0, s, O.parts, R.n, loss);
