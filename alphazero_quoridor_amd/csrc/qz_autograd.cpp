@@ -60,6 +60,16 @@ qz_policy_terms terms_of(const LossArgs& a) {
     t.entropy_coef = (float)a.ent;
     return t;
 }
+// The graph capture that the current stream records into; 0: none, -1: it cannot be told.
+int64_t capture_of(const Tensor& z) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream_of(z)), &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return -1;
+    }
+    return status == hipStreamCaptureStatusNone ? 0 : (int64_t)id;
+}
 Tensor scratch(const Tensor& z, int64_t bytes) { return at::empty({bytes > 0 ? bytes : 1}, z.options().dtype(at::kByte)); }
 
 // ---- log-probabilities.  -> logp, entropy (undefined unless asked for), statistics (undefined unless asked for)
@@ -137,7 +147,8 @@ LossOut run_loss(const Tensor& z, const LossArgs& a, bool want_grad) {
     return o;
 }
 // The forward pass writes the gradient for an upstream factor of 1 beside the loss (one pass over the logits for both); the backward
-// pass hands it out, or computes it again where the factor is another or it was handed out before.
+// pass hands it out, or computes it again where the factor is another, it was handed out before, or the backward pass is recorded into
+// a graph that does not hold the forward pass: its replays would all find what the forward pass wrote once.
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     static variable_list forward(AutogradContext* ctx, const Tensor& z, const LossArgs& a) {
         LossOut o = run_loss(z, a, true);
@@ -146,6 +157,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         ctx->saved_data["coef"] = std::vector<double>{a.lo, a.hi, a.kl, a.ent};
         ctx->saved_data["grad"] = o.grad;
         ctx->saved_data["ws"] = o.ws;
+        ctx->saved_data["capture"] = capture_of(z);
         ctx->mark_non_differentiable({o.logp, o.kl, o.entropy});
         ctx->set_materialize_grads(false);
         return {o.loss, o.logp, o.kl, o.entropy};
@@ -160,9 +172,10 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
         const auto c = ctx->saved_data["coef"].toDoubleVector();
         Tensor grad = ctx->saved_data["grad"].toTensor(), ws = ctx->saved_data["ws"].toTensor();
         ctx->saved_data["grad"] = Tensor();
-        const bool kept = grad.defined();
+        const int64_t capture = capture_of(z);
+        const bool kept = grad.defined() && capture >= 0 && capture == ctx->saved_data["capture"].toInt();
         const int64_t bytes = qz_policy_workspace(z.size(0), (int)z.size(1));
-        if (!kept) {  // a second backward pass: computed again, with a workspace of its own
+        if (!kept) {  // computed again, with a workspace of its own
             grad = at::empty({z.size(0), z.size(1)}, z.options());
             ws = scratch(z, bytes);
         }

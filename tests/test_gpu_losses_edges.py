@@ -90,3 +90,48 @@ def test_forward_mode_is_refused(gpu_device):
         primal = fwd.unpack_dual(dual).primal
         assert torch.equal(losses.clipped_policy_loss(primal, d["actions"], d["adv"], d["old"]).loss, want)
     assert torch.equal(losses.clipped_policy_loss(d["z"], d["actions"], d["adv"], d["old"]).loss, want)
+
+
+@pytest.mark.parametrize("factor", (1.0, 3.0))
+def test_a_captured_backward_pass_of_an_eager_forward_pass(gpu_device, factor):
+    """The graph holds the backward pass alone: every replay computes the gradient of the logits as they are by then, also after the last
+    one's gradient was changed in place."""
+    from alphazero_quoridor_amd import losses
+
+    sets = [{k: v.to(gpu_device) for k, v in make(50, 140, torch.float32, s).items()} for s in (1, 2)]
+    fixed = {k: v for k, v in sets[0].items() if k != "z"}
+
+    def want(z):
+        return losses.policy_loss_and_grad(z, fixed["actions"], fixed["adv"], fixed["old"], legal=fixed["legal"], weights=fixed["w"] * factor)[1]
+
+    side, leaf = torch.cuda.Stream(), torch.zeros((50, 140), device=gpu_device, requires_grad=True)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = leaf + sets[0]["z"]
+        out = losses.clipped_policy_loss(z, fixed["actions"], fixed["adv"], fixed["old"], legal=fixed["legal"], weights=fixed["w"])
+    torch.cuda.synchronize()
+    graph, up = torch.cuda.CUDAGraph(), torch.tensor(factor, device=gpu_device)
+    with torch.cuda.graph(graph, stream=side):
+        grad = torch.autograd.grad(out.loss, z, up, retain_graph=True)[0]
+        grad.mul_(0.5)
+    for k in (0, 0, 1, 1, 0):
+        z.detach().copy_(sets[k]["z"])
+        e = 0.5 * want(z.detach())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float((grad - e).abs().max()) <= 8 * 2.0 ** -24 * (1 + float(e.abs().max())), k  # (the weights carry the factor there: one rounding each)
+        (grad + 1).sum()  # eager work between the replays
+    # the forward pass captured too, in a graph of its own
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first, stream=side):
+        z2 = leaf + sets[0]["z"]
+        out2 = losses.clipped_policy_loss(z2, fixed["actions"], fixed["adv"], fixed["old"], legal=fixed["legal"], weights=fixed["w"])
+    with torch.cuda.graph(second, stream=side):
+        grad2 = torch.autograd.grad(out2.loss, z2, up, retain_graph=True)[0]
+        grad2.mul_(0.5)
+    first.replay()
+    e = 0.5 * want(sets[0]["z"])
+    for _ in range(3):
+        second.replay()
+        torch.cuda.synchronize()
+        assert float((grad2 - e).abs().max()) <= 8 * 2.0 ** -24 * (1 + float(e.abs().max()))
