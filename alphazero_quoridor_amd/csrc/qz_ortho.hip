@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void k_ns_split(Mats M) {
         __syncthreads();
     }
     const double norm = sqrt(sh[0]);
-    const float inv = (float)(1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm));
+    const double inv = 1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm);  // (as a float32 it loses its digits from a norm of 2^126 on)
     const bool tall = m.rows > m.cols;
     const void* src = M.o.muon ? (const void*)m.xt1 : m.update;
     const int64_t ld = M.o.muon ? m.cols : m.ld;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void k_ns_split(Mats M) {
     const int c = threadIdx.x & 63;
     for (int r = threadIdx.x >> 6; r < 64; r += 4) {
         float v = 0.f;
-        if (rr0 + r < m.rows && cc0 + c < m.cols) v = load_elem(src, (int64_t)(rr0 + r) * ld + cc0 + c, dtype) * inv;
+        if (rr0 + r < m.rows && cc0 + c < m.cols) v = (float)((double)load_elem(src, (int64_t)(rr0 + r) * ld + cc0 + c, dtype) * inv);
         if (tall) tile[c][r] = v;  // tile[s][l]
         else tile[r][c] = v;
     }
@@ -668,7 +668,7 @@ __device__ __forceinline__ void strip_first(const Mats& M, const Mat& m, int str
         __syncthreads();
     }
     const double norm = sqrt(sm.sum[0]);
-    const float inv = (float)(1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm));
+    const double inv = 1.0 / (norm < (double)NORM_FLOOR ? (double)NORM_FLOOR : norm);
     __syncthreads();
     const bool tall = m.rows > m.cols;
     const void* src = M.o.muon ? (const void*)m.xt1 : m.update;
@@ -684,7 +684,7 @@ __device__ __forceinline__ void strip_first(const Mats& M, const Mat& m, int str
             for (int e = 0; e < 4; e++) {
                 const int si = s0 + 16 * q + e;
                 v[q][e] = 0.f;
-                if (si < smax && l0 + l < lmax) v[q][e] = load_elem(src, tall ? (int64_t)(l0 + l) * ld + si : (int64_t)si * ld + l0 + l, dtype) * inv;
+                if (si < smax && l0 + l < lmax) v[q][e] = (float)((double)load_elem(src, tall ? (int64_t)(l0 + l) * ld + si : (int64_t)si * ld + l0 + l, dtype) * inv);
             }
 #pragma unroll
         for (int q = 0; q < 4; q++) strip_keep<S>(sm, m.xt0, plane, l0, l, s0 + 16 * q, v[q]);

@@ -1,6 +1,4 @@
 """Orthogonalised updates (optim.py, csrc/qz_ortho.hip): what is refused, and the ends of the number range."""
-import math
-
 import pytest
 import torch
 
@@ -27,3 +25,16 @@ def test_derivatives_of_an_orthogonalised_update_are_refused(gpu_device):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 optim.orthogonalize(x)
         assert torch.equal(optim.orthogonalize(fwd.unpack_dual(dual).primal), want)
+
+
+@pytest.mark.parametrize("shape", ((4, 30), (64, 80), (100, 128), (140, 150), (520, 600)), ids=lambda s: "%dx%d" % s)
+def test_norms_near_the_end_of_float32(gpu_device, shape):
+    """Entries of up to 3e38, whose norm lies beyond float32: the result is, bit for bit, that of the same update times 2^-120.  Squares, their
+    sum, its root and its reciprocal, all in float64, scale by powers of two exactly, and so X_0 = U / |U| comes out the same."""
+    from alphazero_quoridor_amd import optim
+
+    g = torch.Generator().manual_seed(shape[0])
+    u = (torch.rand(shape, generator=g) * 2 - 1).to(gpu_device)
+    big = u * (2.0 ** 127 * 1.7)
+    assert float(big.double().norm()) > 2.0 ** 126 and bool(torch.isfinite(big).all())
+    assert torch.equal(optim.orthogonalize(big), optim.orthogonalize(big * 2.0 ** -120))
