@@ -1107,13 +1107,14 @@ static int policy_rows(const qz_policy_rows* r, PolicyRows* out) {
     if (r->legal_kind < QZ_LEGAL_ALL || r->legal_kind > QZ_LEGAL_BYTES) return fail(QZ_E_INVALID, "unknown legal_kind %d", r->legal_kind);
     if (r->n > 0 && (!r->logits || !r->actions || (r->legal_kind != QZ_LEGAL_ALL && !r->legal))) return fail(QZ_E_INVALID, "null logits, actions or legal set");
     if (r->n > 1 && r->ld < 0) return fail(QZ_E_INVALID, "negative row stride");
-    if (r->legal_kind == QZ_LEGAL_BITS && r->legal_ld < 0) return fail(QZ_E_INVALID, "negative row stride of the legal set");
+    if (r->legal_kind != QZ_LEGAL_ALL && r->legal_ld < 0) return fail(QZ_E_INVALID, "negative row stride of the legal set");
     *out = PolicyRows{r->logits, r->ld, r->n, r->actions, r->legal, r->legal_ld, r->legal_kind, r->dtype, r->n_actions};
     return 0;
 }
 static int policy_terms(const qz_policy_rows* r, const qz_policy_terms* t, PolicyTerms* out) {
     if (!t) return fail(QZ_E_INVALID, "null terms");
     if (r->n > 0 && (!t->advantages || !t->old_logp)) return fail(QZ_E_INVALID, "null advantages or old_logp");
+    if (t->ref_logits && t->ref_ld < 0) return fail(QZ_E_INVALID, "negative row stride of the frozen policy's logits");
     if (t->ref_logits && t->ref_logp) return fail(QZ_E_INVALID, "ref_logits and ref_logp exclude each other");
     if (!(t->clip_low >= 0.f) || !(t->clip_low <= 1.f) || !(t->clip_high >= 0.f)) return fail(QZ_E_INVALID, "clip range [1 - %g, 1 + %g]", t->clip_low, t->clip_high);
     *out = PolicyTerms{t->advantages, t->old_logp, t->ref_logp, t->weights, t->ref_logits, t->ref_ld, t->clip_low, t->clip_high, t->kl_coef, t->entropy_coef,

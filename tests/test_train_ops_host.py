@@ -155,3 +155,15 @@ def test_chained_optimisers_step_and_keep_their_state():
     assert again.param_groups[1]["lr"] == 0.5 and len(again.optimizers[1].state) == 1
     with pytest.raises(ValueError):
         again.load_state_dict({"optimizers": []})
+
+
+def test_negative_strides_are_refused():
+    """A negative stride of the legal set's bytes or of the frozen policy's logits would read before their start."""
+    L, p = lib(), 1 << 20
+    for r, t in ((rows(legal=p, legal_kind=2, legal_ld=-140), terms()), (rows(legal=p, legal_kind=1, legal_ld=-5), terms()), (rows(), terms(ref_logits=p, ref_ld=-140))):
+        assert L.qz_policy_loss(C.byref(r), C.byref(t), p, p, p, p, p, 140, p, BIG, None) == _cabi.E_INVALID, _cabi.load().qz_last_error()
+        assert L.qz_policy_loss_backward(C.byref(r), C.byref(t), p, 0, p, 140, p, BIG, None) == _cabi.E_INVALID
+        assert b"stride" in L.qz_last_error()
+    r = rows(legal=p, legal_kind=2, legal_ld=-140)
+    assert L.qz_action_logp(C.byref(r), p, None, None, p, BIG, None) == _cabi.E_INVALID
+    assert L.qz_action_logp_backward(C.byref(r), p, None, p, None, p, 140, None) == _cabi.E_INVALID
