@@ -1168,6 +1168,12 @@ int qz_policy_loss_backward(const qz_policy_rows* rows, const qz_policy_terms* t
     return 0;
 }
 
+static int matrix_size(const qz_matrix& q, int i) {
+    const int64_t top = 1 << 20;
+    if (q.rows < 0 || q.cols < 0 || q.rows > top || q.cols > top || q.rows * q.cols > (1LL << 32))
+        return fail(QZ_E_INVALID, "matrix %d: %lld x %lld is out of range", i, (long long)q.rows, (long long)q.cols);
+    return 0;
+}
 // the list as the kernels' host side takes it; `muon` = the optimiser step's pointers are checked
 static int matrix_list(const qz_matrix* list, int count, int dtype, bool muon, std::vector<OrthoMatrix>* out) {
     if (count < 0 || (count > 0 && !list)) return fail(QZ_E_INVALID, "bad matrix list");
@@ -1175,9 +1181,7 @@ static int matrix_list(const qz_matrix* list, int count, int dtype, bool muon, s
     out->reserve((size_t)count);
     for (int i = 0; i < count; i++) {
         const qz_matrix& q = list[i];
-        const int64_t top = 1 << 20;
-        if (q.rows < 0 || q.cols < 0 || q.rows > top || q.cols > top || q.rows * q.cols > (1LL << 32))
-            return fail(QZ_E_INVALID, "matrix %d: %lld x %lld is out of range", i, (long long)q.rows, (long long)q.cols);
+        if (const int r = matrix_size(q, i)) return r;
         if (q.rows > 0 && q.cols > 0) {
             if (!q.update || q.ld < 0) return fail(QZ_E_INVALID, "matrix %d: null update or negative stride", i);
             if (muon ? (!q.momentum || !q.param) : (!q.out || (q.rows > 1 && q.out_ld < q.cols)))
@@ -1205,7 +1209,10 @@ int64_t qz_orthogonalize_workspace(const qz_matrix* list, int count) {
     if (count <= 0 || !list) return 0;
     try {
         std::vector<OrthoMatrix> q;
-        for (int i = 0; i < count; i++) q.push_back(OrthoMatrix{list[i].rows, list[i].cols, nullptr, 0, nullptr, 0, nullptr, nullptr, 0.f});
+        for (int i = 0; i < count; i++) {
+            if (const int r = matrix_size(list[i], i)) return r;
+            q.push_back(OrthoMatrix{list[i].rows, list[i].cols, nullptr, 0, nullptr, 0, nullptr, nullptr, 0.f});
+        }
         return qzl::ortho_workspace_bytes(q.data(), count, OrthoStep{});
     } catch (const std::bad_alloc&) {
         return fail(QZ_E_OOM, "out of host memory");

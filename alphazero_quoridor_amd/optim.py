@@ -33,6 +33,8 @@ class _List:
         self.count = len(words) // 9
         self.ptr = C.cast(self.words.buffer_info()[0], C.POINTER(_cabi.qz_matrix))
         self.size = _cabi.load().qz_orthogonalize_workspace(self.ptr, self.count)
+        if self.size < 0:
+            _cabi.check(self.size)
         self.ws = torch.empty(max(self.size, 1), dtype=torch.uint8, device=device)
 
 

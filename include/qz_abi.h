@@ -547,7 +547,8 @@ typedef struct {
     const float* lr_dev;            /* [dev][1] or NULL: the learning rate in device memory (captured graphs follow it) */
 } qz_muon_opts;
 /* out <- the Newton-Schulz iterate of update / max(|update|_F, 1e-7) after `steps` (1 .. 16) quintic steps (3.4445, -4.7750,
- * 2.0315): the singular vectors stay, the singular values move towards 1. */
+ * 2.0315): the singular vectors stay, the singular values move towards 1.  workspace: qz_orthogonalize_workspace bytes (negative: an error
+ * code, for a matrix that the calls refuse). */
 int64_t qz_orthogonalize_workspace(const qz_matrix* list /*[host]*/, int count);
 int qz_orthogonalize(const qz_matrix* list /*[host]*/, int count, int dtype, int steps, void* workspace /*[dev]*/, int64_t workspace_bytes,
                      void* stream);

@@ -167,3 +167,21 @@ def test_negative_strides_are_refused():
     r = rows(legal=p, legal_kind=2, legal_ld=-140)
     assert L.qz_action_logp(C.byref(r), p, None, None, p, BIG, None) == _cabi.E_INVALID
     assert L.qz_action_logp_backward(C.byref(r), p, None, p, None, p, 140, None) == _cabi.E_INVALID
+
+
+def test_the_workspace_of_a_matrix_out_of_range_is_refused():
+    """A caller that allocates what it is told must not be told terabytes for a matrix that the call itself refuses (or what is left of
+    a size past 64 bits)."""
+    L = lib()
+    for rows_, cols in ((1 << 31, 1), (1, (1 << 20) + 1), (1 << 20, 1 << 20), (1 << 62, 1 << 62), (-1, 5)):
+        arr = (_cabi.qz_matrix * 2)(_cabi.qz_matrix(8, 9), _cabi.qz_matrix(rows_, cols))
+        assert L.qz_orthogonalize_workspace(arr, 2) == _cabi.E_INVALID and b"out of range" in L.qz_last_error()
+
+
+def test_python_asks_for_no_memory_for_a_matrix_out_of_range(monkeypatch):
+    from alphazero_quoridor_amd import optim
+
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: pytest.fail("allocated"))
+    with pytest.raises(_cabi.QzError) as e:
+        optim._List([1 << 31, 1, 1 << 20, 1, 1 << 20, 1, 0, 0, 0], torch.device("cpu"))
+    assert e.value.code == _cabi.E_INVALID
