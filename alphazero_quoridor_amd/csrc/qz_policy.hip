@@ -9,7 +9,8 @@
 //   L = w [ -min(r A, clip(r, 1 - lo, 1 + hi) A) + beta KL - eta H ]
 //   KL over a frozen policy's logits: sum q (log q - log p), computed as sum q (e^x - 1 - x), x = log p - log q: every
 //   term is >= 0 and an error of lse cancels to first order, where the plain sum loses all digits of a small KL.
-//   KL from the frozen policy's log-probability of a alone: e^x - 1 - x with x = log q(a) - log p(a).
+//   From the frozen policy's log-probability of a alone: e^x - 1 - x with x = log q(a) - log p(a), whose mean over actions drawn from p is
+//   KL(p || q), the other direction.
 //   dL/dz_j = w [ c (delta_ja - p_j) + beta (p_j - q_j) + eta p_j (log p_j + H) ],
 //   c = -A r where the ratio is not clipped, minus beta (e^x - 1) for the second form of KL.
 // A row whose action is negative, out of range, illegal or has a logit of -inf is LEFT OUT: zero loss, gradient, KL and

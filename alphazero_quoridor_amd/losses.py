@@ -26,7 +26,7 @@ _BYTES = (torch.bool, torch.uint8)
 class PolicyLoss(NamedTuple):
     loss: torch.Tensor     # scalar float32, the only differentiable member
     logp: torch.Tensor     # log pi(a), float32, one per decision; the same for the others
-    kl: torch.Tensor       # KL term of every decision (0 without a frozen policy)
+    kl: torch.Tensor       # KL term of every decision (0 without a frozen policy); which one: see clipped_policy_loss
     entropy: torch.Tensor
 
 
@@ -210,8 +210,9 @@ def clipped_policy_loss(logits, actions, advantages, old_logp, legal: Optional[t
     """sum_i w_i [ -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef KL - entropy_coef H ] with r = exp(log pi(a) - old_logp).
 
     weights: w_i (default 1 / n each; 0 leaves a decision out of the loss).  clip: one number, or (low, high).
-    KL(frozen || pi) over ref_logits (same shape and type as the logits), or estimated from ref_logp, the frozen policy's
-    log-probability of the action, as e^x - 1 - x with x = ref_logp - log pi(a).
+    The KL term with ref_logits (same shape and type as the logits): KL(frozen || pi).  With ref_logp, the frozen policy's
+    log-probability of the action: e^x - 1 - x with x = ref_logp - log pi(a), which estimates the other direction, KL(pi || frozen),
+    where actions are drawn from pi.  One kl_coef does not weigh the two alike.
     Differentiable in ``logits``; memory for their gradient is taken in the forward pass."""
     args, lead = _loss_arguments(logits, actions, advantages, old_logp, legal, weights, ref_logits, ref_logp, clip, kl_coef, entropy_coef)
     _refuse_captured_leaf(logits)

@@ -502,9 +502,10 @@ typedef struct {
 typedef struct {
     const float* advantages;        /* [dev][n]                                                        */
     const float* old_logp;          /* [dev][n]  log-probability under the policy that acted           */
-    const float* ref_logp;          /* [dev][n] or NULL: KL estimated from the frozen policy's log-probability of the action */
+    const float* ref_logp;          /* [dev][n] or NULL: the frozen policy's log-probability of the action; the KL term is then e^x - 1 - x with
+                                     * x = ref_logp - logp, an estimate of KL(pi || frozen) where actions are drawn from pi */
     const float* weights;           /* [dev][n] or NULL: 1 / n each                                    */
-    const void* ref_logits;         /* [dev] or NULL: KL over the frozen policy's logits (same type)   */
+    const void* ref_logits;         /* [dev] or NULL: the KL term is KL(frozen || pi) over these logits (same type) */
     int64_t ref_ld;
     float clip_low, clip_high;      /* the ratio is clipped to [1 - clip_low, 1 + clip_high]           */
     float kl_coef, entropy_coef;

@@ -135,3 +135,20 @@ def test_a_captured_backward_pass_of_an_eager_forward_pass(gpu_device, factor):
         second.replay()
         torch.cuda.synchronize()
         assert float((grad2 - e).abs().max()) <= 8 * 2.0 ** -24 * (1 + float(e.abs().max()))
+
+
+def test_which_divergence_the_kl_terms_are(gpu_device):
+    """Over the logits: KL(frozen || pi).  From ref_logp: terms whose mean over actions drawn from pi is KL(pi || frozen).  Every action of one
+    distribution is a decision here, so that the mean is a sum; each term is good to 16 u (1 + |x| + e^x)."""
+    from alphazero_quoridor_amd import losses
+
+    g = torch.Generator().manual_seed(9)
+    z, zq = torch.randn(40, generator=g), torch.randn(40, generator=g)
+    lp, lq = torch.log_softmax(z.double(), 0), torch.log_softmax(zq.double(), 0)
+    rows = dict(logits=z.expand(40, 40).contiguous().to(gpu_device), actions=torch.arange(40, device=gpu_device), advantages=torch.zeros(40, device=gpu_device),
+                old_logp=lp.float().to(gpu_device), kl_coef=1.0)
+    over = losses.clipped_policy_loss(ref_logits=zq.expand(40, 40).contiguous().to(gpu_device), **rows).kl.double().cpu()
+    taken = losses.clipped_policy_loss(ref_logp=lq.float().to(gpu_device), **rows).kl.double().cpu()
+    tol = 16 * 2.0 ** -24 * float((lp.exp() * (1 + (lq - lp).abs() + (lq - lp).exp())).sum())
+    assert float((over - (lq.exp() * (lq - lp)).sum()).abs().max()) <= 8 * tol
+    assert abs(float((lp.exp() * taken).sum() - (lp.exp() * (lp - lq)).sum())) <= tol
