@@ -8,7 +8,8 @@
 //   A = X X^T (symmetric: the lower tiles, mirrored);  B = b A + c A A (A is symmetric, so A A = A A^T; symmetric again);
 //   X'^T = a X^T + X^T B (B symmetric): rows of X^T against rows of B.  So X is kept in both orientations.
 // float32 accuracy on the fp16 matrix pipe: every value is hi + lo, two fp16 numbers of the value times 4096 (a 22-bit
-// significand; all entries are below 4 in magnitude, so 4096 keeps hi in range and lo out of the subnormals down to 2^-15), and a
+// significand; all entries are below 4 in magnitude, so 4096 keeps hi in range and lo out of the subnormals down to 2^-15; an entry below
+// that is kept to 2^-36 absolute, so a row far smaller than the rest keeps fewer digits than float32 would give it), and a
 // product is hi hi + hi lo + lo hi with float32 accumulation, whatever the result's type: hi hi alone leaves a bfloat16 result up to
 // 2.9e-3 off float64 (updates of flat or sparse spectra, 1,024 x 4,096) where its own rounding is 1.66e-3.
 #include <hip/hip_bf16.h>
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(256) void k_ns_split(Mats M) {
 }
 
 // ---- C = P Q^T, one TxT tile per workgroup of four waves (2 x 2), K in steps of 32 through LDS.
-// Measured at 4096^3: the product with X 465 us (885 TFLOP/s of fp16 products; this card's library product reaches 1,163), the matrix
+// Measured at 4096^3: the product with X 478 us (862 TFLOP/s of fp16 products; this card's library product reaches 1,163), the matrix
 // pipe busy for half of the cycles at 1.9 GHz, LDS reads and writes about as long; no bank conflicts; L2 hits 88 %.
 // LDS rows are 64 bytes = four 16-byte chunks; chunk q of row r sits at q ^ ((r >> 2) & 3), so that the sixteen lanes that one
 // pass of a 16-byte read serves fall on sixteen different bank groups.
@@ -228,7 +229,8 @@ __device__ __forceinline__ void tile_lower(int w, int t, int& ti, int& tj) {  //
 }
 
 // Four rows of one column of a symmetric product: A = P P^T as it is, or b A + c A A (A[row][col] = A[col][row]), as planes, and the
-// mirrored tile (a tile on the diagonal holds both halves already, equal bit for bit).
+// mirrored tile (a tile on the diagonal computes both halves; they may differ in the last bit, lo hi and hi lo being added the other way
+// round there).
 template <int KIND>
 __device__ __forceinline__ void store_symmetric(const Mat& m, bool mirror, int row, int col, float (&v)[4]) {
     const int64_t plane = (int64_t)m.sp * m.sp;
@@ -262,7 +264,8 @@ __device__ __forceinline__ void store_symmetric(const Mat& m, bool mirror, int r
 // across[column][row], and to along[row][column] too unless the tile lies on the diagonal of a symmetric product.  Through 8 KB of LDS
 // that the stages have left: float32 sums in, rows out (the old values, laid out like `along`, in on the way), then the halves in once
 // more and columns out.  Every access to memory is 16 bytes a lane and 64 bytes or more a row; straight from the accumulators it is 2
-// bytes a lane for rows and 8 bytes a column (1024 x 4096 and its transpose: 56 us a product, 39 us so).
+// bytes a lane for rows and 8 bytes a column (X' of 1024 x 4096 and its transpose: 92 us, 79 us so; of four 1024 x 1024 with them: 149 and
+// 120 us).
 template <bool OLD>
 __device__ __forceinline__ void store_both(const floatx16 (&acc)[2], char* mine, int rb, int cb, const _Float16* old, _Float16* along, _Float16* across,
                                            int64_t plane, int64_t ld_along, int64_t ld_across, float c_old, float c_new, bool both) {
@@ -1080,18 +1083,20 @@ template <int KIND>
 void run_gemm(Mats& M, bool may128, float* partial, int odd, int last, hipStream_t s) {
     int tiles = may128 ? set_starts<KIND>(M, 128, 0) : 0;
     // Tiles of 128 read half as much through LDS per product, tiles of 64 give four times the workgroups.  B = b A + c A A, whose sum is
-    // short, takes the larger ones where there is one for every other CU (two 1024 x 1024 products, 72 tiles: 15 us in tiles of 64, 23 us
-    // in tiles of 128; six, 216 tiles: 52 us and 45 us); the others, unless there would be next to none (A of two 1024 x 4096: 35 us in
-    // tiles of 64, 33 us in tiles of 128 split along the sum).
+    // short, takes the larger ones where there is one for every other CU (two 1024 x 1024 products, 72 tiles: 27 us in tiles of 64, 39 us
+    // in tiles of 128; six, 216 tiles: 52 us and 45 us); the others, unless there would be next to none (A of two 1024 x 4096: 78 us in
+    // tiles of 64, 59 us in tiles of 128 split along the sum; of two 1024 x 1024, whose sum is too short to split, 23 and 32 us).
     if (tiles < (KIND == KIND_POLY ? 128 : 32)) {
         tiles = set_starts<KIND>(M, 64, 0);
-        if (KIND == KIND_APPLY) hipLaunchKernelGGL((k_ns_gemm<64, KIND, 4>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
+        if constexpr (KIND == KIND_APPLY) hipLaunchKernelGGL((k_ns_gemm<64, KIND, 4>), dim3(tiles), dim3(256), 0, s, M, Part{0, 0, odd, last, 0, nullptr});
         else run_symmetric<KIND, 64>(M, tiles, partial, odd, last, s);
         return;
     }
-    if (KIND != KIND_APPLY && tiles <= SLOTS) {
-        run_symmetric<KIND, 128>(M, tiles, partial, odd, last, s);
-        return;
+    if constexpr (KIND != KIND_APPLY) {
+        if (tiles <= SLOTS) {
+            run_symmetric<KIND, 128>(M, tiles, partial, odd, last, s);
+            return;
+        }
     }
     // what is left over a multiple of the slots runs in quarters, if it is less than half a round
     const int rest = tiles % SLOTS, head = tiles > SLOTS && rest * 2 < SLOTS ? tiles - rest : tiles;

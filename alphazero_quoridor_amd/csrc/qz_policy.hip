@@ -989,7 +989,8 @@ bool few(int64_t n) { return n <= 256; }
 // The smallest workgroup whose registers hold the row: 8,192 x 32,768 bfloat16 with a frozen policy 410 us, 452 us read twice; without
 // one 206 and 250 us; 2,048 x 4,000 23 and 32 us.  Past 512 threads of 8 chunks the row is read twice: a workgroup of 1,024 would have
 // a CU to itself, and nothing to cover its loads with (2,048 x 50,001: 315 us, 226 us read twice) -- but for one input with a mask, whose
-// second reading costs more (2,047 x 50,001 with a byte mask: 180 us, 191 us read twice).
+// second reading costs more (2,047 x 50,001 with a byte mask: 180 us, 191 us read twice).  A mask and a frozen policy together at 2,049 to
+// 4,096 chunks need 80 bytes a lane of scratch: 8,192 x 32,768 bfloat16 669 us.
 template <typename T>
 void wide_loss(const PolicyRows& R, const PolicyTerms& P, const PolicyOut& O, unsigned wgs, hipStream_t s) {
     const int chunks = (R.a + Elem<T>::V - 1) / Elem<T>::V;
