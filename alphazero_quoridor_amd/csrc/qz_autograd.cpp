@@ -24,6 +24,8 @@ void refuse_tangents(std::initializer_list<Tensor> inputs) {
     for (const Tensor& t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "the policy losses have no forward-mode derivative");
 }
+// (a lazily negated view's memory holds the values of the other sign)
+Tensor plain(const Tensor& t) { return t.resolve_neg().contiguous(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? QZ_F32 : t.scalar_type() == at::kBFloat16 ? QZ_BF16 : QZ_F16; }
@@ -102,7 +104,7 @@ struct ActionLogp : torch::autograd::Function<ActionLogp> {
         refuse_twice();
         const auto saved = ctx->get_saved_variables();
         const Tensor &z = saved[0], &h = saved[4];
-        const Tensor dlogp = up[0].defined() ? up[0].contiguous() : Tensor(), dh = up.size() > 1 && up[1].defined() ? up[1].contiguous() : Tensor();
+        const Tensor dlogp = up[0].defined() ? plain(up[0]) : Tensor(), dh = up.size() > 1 && up[1].defined() ? plain(up[1]) : Tensor();
         Tensor grad;
         if (dlogp.defined() || dh.defined()) {
             const c10::DeviceGuard guard(z.device());
@@ -179,7 +181,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
             grad = at::empty({z.size(0), z.size(1)}, z.options());
             ws = scratch(z, bytes);
         }
-        const Tensor upstream = up[0].contiguous();
+        const Tensor upstream = plain(up[0]);
         const LossArgs a = {s[1], s[2], s[3], s[4], s[5], s[6], s[7], ctx->saved_data["kind"].toInt(), c[0], c[1], c[2], c[3]};
         const qz_policy_rows r = rows_of(z, a.actions, a.legal, a.kind);
         const qz_policy_terms t = terms_of(a);

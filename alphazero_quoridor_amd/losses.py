@@ -37,6 +37,11 @@ def _gpu(t, name):
         raise _cabi.QzError(_cabi.E_NO_DEVICE, "%s is on %s; this package has no CPU path" % (name, t.device))
 
 
+def _plain(t):
+    """A lazily negated view (the imaginary part of a conjugate) as the values it stands for: its memory holds the others."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _same_device(t, device, name):
     _gpu(t, name)
     if t.device != device:
@@ -52,6 +57,7 @@ def _rows_of(logits, name="logits"):
         raise ValueError("%s: at least one action is needed, got the shape %s" % (name, tuple(logits.shape)))
     if logits.shape[-1] > 1 << 30:
         raise ValueError("%s: %d actions, at most 2^30 are supported" % (name, logits.shape[-1]))
+    logits = _plain(logits)
     return logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
 
 
@@ -71,6 +77,7 @@ def _vector(t, lead, device, name):
         raise TypeError("%s must be floating point" % name)
     if tuple(t.shape) != tuple(lead):
         raise ValueError("%s has the shape %s, %s is needed" % (name, tuple(t.shape), tuple(lead)))
+    t = _plain(t)
     if t.dtype is torch.float32 and t.dim() == 1 and t.is_contiguous():
         return t
     return t.to(torch.float32).reshape(-1).contiguous()
@@ -82,6 +89,7 @@ def _actions(t, lead, device):
         raise TypeError("actions must be integers")
     if tuple(t.shape) != tuple(lead):
         raise ValueError("actions have the shape %s, %s is needed" % (tuple(t.shape), tuple(lead)))
+    t = _plain(t)
     if t.dtype is torch.int64 and t.dim() == 1 and t.is_contiguous():
         return t
     return t.to(torch.int64).reshape(-1).contiguous()

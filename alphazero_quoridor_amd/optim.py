@@ -12,7 +12,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _cabi
-from .losses import DTYPES, _call, _gpu
+from .losses import DTYPES, _call, _gpu, _plain
 
 
 def _matrix(t, name):
@@ -20,6 +20,7 @@ def _matrix(t, name):
     _gpu(t, name)
     if t.dim() < 2:
         raise ValueError("%s: a matrix is needed, got the shape %s" % (name, tuple(t.shape)))
+    t = _plain(t)
     if t.dim() > 2:
         t = t.reshape(t.shape[0], math.prod(t.shape[1:]))  # (no -1: a side may be zero)
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()

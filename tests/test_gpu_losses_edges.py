@@ -152,3 +152,27 @@ def test_which_divergence_the_kl_terms_are(gpu_device):
     tol = 16 * 2.0 ** -24 * float((lp.exp() * (1 + (lq - lp).abs() + (lq - lp).exp())).sum())
     assert float((over - (lq.exp() * (lq - lp)).sum()).abs().max()) <= 8 * tol
     assert abs(float((lp.exp() * taken).sum() - (lp.exp() * (lp - lq)).sum())) <= tol
+
+
+def test_negated_views(gpu_device):
+    """The imaginary part of a conjugate is a view whose memory holds the other sign; a single element, or a single column, of one counts as
+    contiguous."""
+    from alphazero_quoridor_amd import losses
+
+    c = torch.randn((1, 8), dtype=torch.complex64, generator=torch.Generator().manual_seed(2)).to(gpu_device).conj()
+    z, v = c.real.contiguous(), c[:, 3].imag
+    assert v.is_neg() and v.is_contiguous()
+    act = torch.tensor([2], device=gpu_device)
+    args = dict(advantages=v, old_logp=c[:, 4].imag, weights=c[:, 5].imag, ref_logp=c[:, 6].imag, kl_coef=0.1)
+    plain = {k: x.clone().resolve_neg() if torch.is_tensor(x) else x for k, x in args.items()}
+    for a, b in zip(losses.policy_loss_and_grad(z, act, **args)[0], losses.policy_loss_and_grad(z, act, **plain)[0]):
+        assert torch.equal(a, b)
+    many = torch.randn((4, 8), dtype=torch.complex64, generator=torch.Generator().manual_seed(3)).to(gpu_device).conj().imag
+    for logits in (many, many.t(), torch._neg_view(z.expand(4, 8).contiguous())):
+        a = torch.arange(logits.shape[0], device=gpu_device) % logits.shape[1]
+        assert logits.is_neg() and torch.equal(losses.action_logp(logits, a), losses.action_logp(logits.resolve_neg().contiguous(), a))
+    # upstream gradients
+    x = z.clone().requires_grad_(True)
+    for f, up in ((lambda: losses.action_logp(x, act), c[:, 1].imag), (lambda: losses.clipped_policy_loss(x, act, c.real[:, 1], c.real[:, 2]).loss, c[0, 1].imag)):
+        assert up.is_neg()
+        assert torch.equal(torch.autograd.grad(f(), x, up)[0], torch.autograd.grad(f(), x, up.resolve_neg().clone())[0])

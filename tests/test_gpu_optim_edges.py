@@ -38,3 +38,18 @@ def test_norms_near_the_end_of_float32(gpu_device, shape):
     big = u * (2.0 ** 127 * 1.7)
     assert float(big.double().norm()) > 2.0 ** 126 and bool(torch.isfinite(big).all())
     assert torch.equal(optim.orthogonalize(big), optim.orthogonalize(big * 2.0 ** -120))
+
+
+def test_negated_views(gpu_device):
+    """The imaginary part of a conjugate is a view whose memory holds the other sign; nothing of it need be copied where it has one column."""
+    from alphazero_quoridor_amd import optim
+
+    c = torch.randn((30, 40), dtype=torch.complex64, generator=torch.Generator().manual_seed(2)).to(gpu_device).conj()
+    for u in (c.imag, c[:, :1].imag, c[:1].imag.t(), torch._neg_view(c.real.contiguous())):
+        assert u.is_neg()
+        assert torch.equal(optim.orthogonalize(u), optim.orthogonalize(u.resolve_neg().contiguous()))
+    p, q = (torch.nn.Parameter(torch.zeros((30, 1), device=gpu_device)) for _ in range(2))
+    p.grad, q.grad = c[:, :1].imag, c[:, :1].imag.resolve_neg().contiguous()
+    for x in (p, q):
+        optim.Muon([x], lr=0.1).step()
+    assert torch.equal(p, q)
