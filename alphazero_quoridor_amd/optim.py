@@ -65,7 +65,7 @@ def orthogonalize(update, steps=5):
     for u in updates:
         _gpu(u, "update")
         _constant(u, "update")
-        m = _matrix(u.detach(), "update")
+        m = _matrix(u, "update")
         if u.dtype not in DTYPES:
             raise TypeError("update: %s is not one of float32, bfloat16, float16" % u.dtype)
         o = torch.empty(u.shape, dtype=u.dtype, device=u.device)
